@@ -94,10 +94,16 @@ struct h3b_ctx {
     cudaError_t e = cudaSetDevice(device);
     return e == cudaSuccess ? 0 : fail_cuda("cudaSetDevice", e);
   }
-  // Called before every launch: opens the timed region of the next wait.
+  // Called before every launch: opens the timed region of the next wait. A launch that is being captured into a graph
+  // belongs to no timed region: an event recorded into the graph could not be read by the next wait.
   int before_launch(cudaEvent_t *prof_start) {
     if (make_current()) return -1;
     cudaError_t e;
+    if (profile || !timing_open) {
+      cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+      if ((e = cudaStreamIsCapturing(stream, &capture)) != cudaSuccess) return fail_cuda("cudaStreamIsCapturing", e);
+      if (capture != cudaStreamCaptureStatusNone) return profile ? fail("profile mode times every launch: it cannot be captured") : 0;
+    }
     if (profile) {
       if ((e = cudaEventRecord(ev_start, stream)) != cudaSuccess) return fail_cuda("cudaEventRecord", e);
       *prof_start = ev_start;
@@ -269,6 +275,7 @@ h3b_ctx *h3b_open(int device) {
   ctx->encode = reinterpret_cast<EncodeTiledFn>(fn);
   if ((e = h3b::gemm_configure(device)) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
   if ((e = h3b::gemm_pair_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
+  if ((e = h3b::gemm_f8_small_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
   ctx->pair_stages = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, false);
   ctx->pair_stages_staged = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, true);
   ctx->pair_clusters = ctx->pair_stages >= 2 ? h3b::gemm_pair_max_clusters(ctx->pair_stages) : 0;
@@ -818,6 +825,95 @@ int h3b_gemm_w8a8_lora_noalloc(h3b_ctx *ctx, const int8_t *A, int64_t a_stride, 
     return -1;
   return gemm_enqueue(ctx, A, a_stride, W, w_stride, sw, sa, bias, C, c_dtype, c_stride, M, N, K, T, R, lora_B, b_stride,
                       R, lora_ranges, false);
+}
+
+// ---- block-scaled e4m3 -------------------------------------------------------------------------------------------------
+static int float_size(int dtype) { return dtype == H3B_F32 ? 4 : (dtype == H3B_F16 || dtype == H3B_BF16) ? 2 : 0; }
+static bool rows_aligned(const void *p, int64_t stride, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * size) % 16 == 0;
+}
+
+int h3b_quant_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, void *out, int64_t out_stride, float *sa,
+                 int64_t sa_stride, int M, int D, int mode) {
+  if (!ctx) return fail("null context");
+  if (!x || !out || !sa) return fail("quant_f8: null tensor argument");
+  if (M <= 0 || D <= 0) return fail("quant_f8: M and D must be positive");
+  if (mode != 0 && mode != 1) return fail("quant_f8: mode must be 0 or 1");
+  const int size = float_size(x_dtype);
+  if (!size) return fail("quant_f8: input type must be bf16, f16 or f32");
+  if (x_stride < (mode == 1 ? 2LL * D : D) || out_stride < D) return fail("quant_f8: x_stride / out_stride smaller than the row");
+  if (sa_stride < M) return fail("quant_f8: sa_stride smaller than M");
+  if (!rows_aligned(x, x_stride, size) || !rows_aligned(out, out_stride, 1))
+    return fail("quant_f8: rows must be 16-byte aligned");
+  if (D > (1 << 28)) return fail("quant_f8: D exceeds 2^28 channels");
+  h3b::QuantF8Launch q;
+  q.x = x; q.out = out; q.sa = sa; q.x_stride = x_stride; q.out_stride = out_stride; q.sa_stride = sa_stride;
+  q.x_dtype = x_dtype; q.M = M; q.D = D; q.gated = mode;
+  cudaEvent_t ps = nullptr;
+  if (ctx->before_launch(&ps)) return -1;
+  return ctx->after_launch("quant_f8 launch", h3b::launch_quant_f8(q, ctx->overlap != 0 && !ctx->profile, ctx->stream));
+}
+
+int h3b_rms_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, const void *y, int y_dtype, int64_t y_stride,
+               void *res, int64_t res_stride, const void *w, int w_dtype, void *out, int64_t out_stride, float *sa,
+               int64_t sa_stride, int M, int D, float eps) {
+  if (!ctx) return fail("null context");
+  if (!x || !w || !out || !sa) return fail("rms_f8: null tensor argument");
+  if ((y != nullptr) != (res != nullptr)) return fail("rms_f8: y and res go together");
+  if (M <= 0 || D <= 0) return fail("rms_f8: M and D must be positive");
+  if (D > h3b::kRmsF8MaxD) return fail("rms_f8: D exceeds the 32768 channels one CTA covers");
+  const int sx = float_size(x_dtype), sy = y ? float_size(y_dtype) : 1;
+  if (!sx || !sy || !float_size(w_dtype)) return fail("rms_f8: x, y and w must be bf16, f16 or f32");
+  if (x_stride < D || out_stride < D || (y && (y_stride < D || res_stride < D)))
+    return fail("rms_f8: a row stride is smaller than the row");
+  if (sa_stride < M) return fail("rms_f8: sa_stride smaller than M");
+  if (!rows_aligned(x, x_stride, sx) || !rows_aligned(out, out_stride, 1) || !rows_aligned(w, 0, 1) ||
+      (y && (!rows_aligned(y, y_stride, sy) || !rows_aligned(res, res_stride, sx))))
+    return fail("rms_f8: rows must be 16-byte aligned");
+  if (!(eps >= 0.0f)) return fail("rms_f8: eps must not be negative");
+  h3b::RmsF8Launch r;
+  r.x = x; r.y = y; r.w = w; r.res = res; r.out = out; r.sa = sa;
+  r.x_stride = x_stride; r.y_stride = y_stride; r.res_stride = res_stride; r.out_stride = out_stride; r.sa_stride = sa_stride;
+  r.x_dtype = x_dtype; r.y_dtype = y_dtype; r.w_dtype = w_dtype; r.M = M; r.D = D; r.eps = eps;
+  cudaEvent_t ps = nullptr;
+  if (ctx->before_launch(&ps)) return -1;
+  return ctx->after_launch("rms_f8 launch", h3b::launch_rms_f8(r, ctx->overlap != 0 && !ctx->profile, ctx->stream));
+}
+
+int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, int64_t sa_stride, const void *W,
+                int64_t w_stride, const float *sw, int64_t sw_stride, const float *bias, void *C, int c_dtype,
+                int64_t c_stride, int M, int N, int K) {
+  if (!ctx) return fail("null context");
+  if (!A || !sa || !W || !sw || !C) return fail("gemm_f8: null tensor argument");
+  if (M <= 0 || N <= 0 || K <= 0) return fail("gemm_f8: M, N and K must be positive");
+  if (!float_size(c_dtype)) return fail("gemm_f8: output type must be bf16, f16 or f32");
+  if (a_stride < K || w_stride < K) return fail("gemm_f8: a_stride / w_stride smaller than K");
+  if (c_stride < N) return fail("gemm_f8: c_stride smaller than N");
+  const int groups = (K - 1) / 128 + 1;
+  if (sa_stride < M || sw_stride < groups) return fail("gemm_f8: sa_stride smaller than M or sw_stride than the scale blocks of a row");
+  if (!rows_aligned(A, a_stride, 1) || !rows_aligned(W, w_stride, 1))
+    return fail("gemm_f8: A and W must be 16-byte aligned with row strides that are multiples of 16 bytes");
+  if (reinterpret_cast<uintptr_t>(C) % float_size(c_dtype) || reinterpret_cast<uintptr_t>(sa) % 4 ||
+      reinterpret_cast<uintptr_t>(sw) % 4 || reinterpret_cast<uintptr_t>(bias) % 4)
+    return fail("gemm_f8: a tensor is not aligned to its elements");
+  h3b::GemmF8Launch g;
+  memset(&g, 0, sizeof g);
+  g.sa = sa; g.sw = sw; g.bias = bias; g.c = C; g.c_stride = c_stride; g.sa_stride = sa_stride; g.sw_stride = sw_stride;
+  g.c_dtype = c_dtype; g.M = M; g.N = N; g.K = K;
+  g.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  g.m_tiles = (M - 1) / g.nt + 1;
+  g.split = 1;
+  g.overlap = (ctx->overlap != 0 && !ctx->profile) ? 1 : 0;
+  g.status = ctx->status_dev;
+  if (((N - 1LL) / 128 + 1) * g.m_tiles * g.split > 0x7FFFFFFFLL) return fail("gemm_f8: too many tiles for one launch");
+  const CUtensorMap *m;
+  if (!(m = ctx->tensor_map(A, h3b::kDtypeI8, K, M, a_stride, 128, g.nt, 128))) return -1;
+  g.map_a = *m;
+  if (!(m = ctx->tensor_map(W, h3b::kDtypeI8, K, N, w_stride, 128, 128, 128))) return -1;
+  g.map_w = *m;
+  cudaEvent_t ps = nullptr;
+  if (ctx->before_launch(&ps)) return -1;
+  return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_small(g, ctx->stream));
 }
 
 int h3b_selftest_expire_wait(h3b_ctx *ctx) {

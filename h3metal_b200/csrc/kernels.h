@@ -8,7 +8,7 @@
 namespace h3b {
 
 // Element types as the C ABI numbers them (include/h3b200.h).
-enum Dtype : int { kDtypeF32 = 0, kDtypeF16 = 1, kDtypeBf16 = 2, kDtypeI8 = 3, kDtypeI32 = 4 };
+enum Dtype : int { kDtypeF32 = 0, kDtypeF16 = 1, kDtypeBf16 = 2, kDtypeI8 = 3, kDtypeI32 = 4, kDtypeF8 = 5 };
 constexpr int kMaxPeers = 8;  // GPUs of one node that may share a row-parallel layer
 
 void rot_q8_geometry(int D, int threads_target, int *ch, int *threads);
@@ -162,5 +162,42 @@ int gemm_pair_pick_stages(size_t smem_optin, bool staged_stores);
 cudaError_t gemm_pair_configure();
 int gemm_pair_max_clusters(int stages);
 cudaError_t launch_gemm_w8a8_pair(const GemmLaunch &g, int stages, int clusters, cudaStream_t stream);
+
+// ---- block-scaled e4m3: codes with one fp32 scale per 128 channels ---------------------------------------------------
+// Activation scales lie group by group, sa[group][sa_stride >= M]; weight scales sw[n / 128][group].
+struct QuantF8Launch {
+  const void *x;        // [M][x_stride] of x_dtype; gated: columns D..2D-1 hold the gates
+  void *out;            // codes [M][out_stride]
+  float *sa;
+  long long x_stride, out_stride, sa_stride;
+  int x_dtype, M, D, gated;
+};
+cudaError_t launch_quant_f8(const QuantF8Launch &q, bool overlap, cudaStream_t stream);
+
+struct RmsF8Launch {
+  const void *x, *y, *w;  // y: added to x first (or null); w [D]
+  void *res;              // x + y in x's type (may be x); unused without y
+  void *out;
+  float *sa;
+  long long x_stride, y_stride, res_stride, out_stride, sa_stride;
+  int x_dtype, y_dtype, w_dtype, M, D;
+  float eps;
+};
+constexpr int kRmsF8MaxD = 32768;
+cudaError_t launch_rms_f8(const RmsF8Launch &r, bool overlap, cudaStream_t stream);
+
+struct GemmF8Launch {
+  CUtensorMap map_a;   // e4m3 [M][K], box nt x 128 bytes, 128-byte swizzle
+  CUtensorMap map_w;   // e4m3 [N][K], box 128 x 128 bytes
+  const float *sa, *sw, *bias;
+  void *c;
+  long long c_stride, sa_stride, sw_stride;
+  int c_dtype, M, N, K;
+  int nt, m_tiles, split;  // rows of A per tile, tiles of that height, CTAs that share K
+  int overlap;
+  int *status;
+};
+cudaError_t gemm_f8_small_configure();
+cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, cudaStream_t stream);
 
 }  // namespace h3b

@@ -125,6 +125,18 @@ __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// ---- small asynchronous copies -----------------------------------------------------------------------------------
+// Four bytes global -> shared, zeros where `ok` is false (the address must be valid all the same).
+__device__ __forceinline__ void cp_async_4(uint32_t dst_smem, const void *src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst_smem), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of this thread's groups are still on their way.
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // ---- tensor memory ----------------------------------------------------------------------------------------------
 // Whole-warp calls. `cols` is a power of two in [32, 512]; the base address is written to shared memory.
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t cols) {
@@ -160,7 +172,8 @@ __device__ __forceinline__ uint64_t umma_smem_desc(uint32_t smem_addr, uint32_t 
 }
 
 // Instruction descriptor, dense, no negation, both operands K-major.
-//   c_format: 0 f16, 1 f32, 2 s32;  ab_format: kind::i8 -> 0 u8, 1 s8;  kind::f16 -> 0 f16, 1 bf16
+//   c_format: 0 f16, 1 f32, 2 s32;  ab_format: kind::i8 -> 0 u8, 1 s8;  kind::f16 -> 0 f16, 1 bf16;
+//   kind::f8f6f4 -> 0 e4m3, 1 e5m2
 __host__ __device__ constexpr uint32_t umma_instr_desc(uint32_t c_format, uint32_t ab_format, uint32_t m, uint32_t n) {
   return (c_format << 4) | (ab_format << 7) | (ab_format << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
@@ -195,6 +208,18 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
       ".reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// e4m3 / e5m2 operands (kind::f8f6f4), fp32 accumulation; one instruction covers 32 channels.
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
       "}\n" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");

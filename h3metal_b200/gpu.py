@@ -29,8 +29,8 @@ import numpy as np
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
-H3B_F32, H3B_F16, H3B_BF16, H3B_I8, H3B_I32 = 0, 1, 2, 3, 4
-_ABI_DTYPE = {"f32": H3B_F32, "f16": H3B_F16, "bf16": H3B_BF16, "i8": H3B_I8, "i32": H3B_I32}
+H3B_F32, H3B_F16, H3B_BF16, H3B_I8, H3B_I32, H3B_F8 = 0, 1, 2, 3, 4, 5
+_ABI_DTYPE = {"f32": H3B_F32, "f16": H3B_F16, "bf16": H3B_BF16, "i8": H3B_I8, "i32": H3B_I32, "f8": H3B_F8}
 _METAL_T = {"half": "f16", "bfloat": "bf16", "float": "f32"}
 
 
@@ -86,6 +86,9 @@ def _signatures():
         "h3b_reduce_dequant_low": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, i64, ctypes.POINTER(vp), i32, i32, i64, i32,
                                          i32, i32, vp, vp, i64]),
         "h3b_reduce_dequant_gated": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, vp, i64]),
+        "h3b_rms_f8": (i32, [vp, vp, i32, i64, vp, i32, i64, vp, i64, vp, i32, vp, i64, vp, i64, i32, i32, ctypes.c_float]),
+        "h3b_quant_f8": (i32, [vp, vp, i32, i64, vp, i64, vp, i64, i32, i32, i32]),
+        "h3b_gemm_f8": (i32, [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i32, i32, i32]),
         "h3b_gemm_tile_n": (i32, [vp, i32, i32]),
         "h3b_gemm_set_policy": (i32, [vp, i32, i32, i32]),
         "h3b_gemm_set_store_mode": (i32, [vp, i32]),
@@ -125,9 +128,9 @@ def _err() -> str:
 
 _NP = {
     "f32": np.float32, "f16": np.float16, "bf16": np.uint16, "i8": np.int8, "u8": np.uint8,
-    "i32": np.int32, "u32": np.uint32, "i16": np.int16, "u16": np.uint16,
+    "i32": np.int32, "u32": np.uint32, "i16": np.int16, "u16": np.uint16, "f8": np.uint8,
 }
-_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "i8": 1, "u8": 1, "i32": 4, "u32": 4, "i16": 2, "u16": 2}
+_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "i8": 1, "u8": 1, "i32": 4, "u32": 4, "i16": 2, "u16": 2, "f8": 1}
 
 
 def _torch():
@@ -138,7 +141,7 @@ def _torch():
 def _torch_dtype(dtype: str):
     t = _torch()
     return {"f32": t.float32, "f16": t.float16, "bf16": t.bfloat16, "i8": t.int8, "u8": t.uint8, "i32": t.int32,
-            "i16": t.int16, "u16": t.uint16, "u32": t.uint32}[dtype]
+            "i16": t.int16, "u16": t.uint16, "u32": t.uint32, "f8": t.float8_e4m3fn}[dtype]
 
 
 @dataclass
@@ -163,6 +166,10 @@ class Tensor:
         return int(math.prod(self.shape) * _SIZE[self.dtype])
 
     @property
+    def numel(self) -> int:
+        return math.prod(self.shape)
+
+    @property
     def ptr(self) -> int:
         return self.buf.handle + self.offset
 
@@ -178,9 +185,11 @@ class Tensor:
     def numpy(self) -> np.ndarray:
         """A host copy of the data, taken after the device has finished the work launched so far.
 
-        bf16 comes back as uint16 bit patterns, as in the reference."""
+        bf16 comes back as uint16 bit patterns, as in the reference; f8 (e4m3 codes) as uint8 bit patterns."""
         t = self.torch()
-        if self.dtype == "bf16":
+        if self.dtype == "f8":
+            t = t.view(_torch().uint8)
+        elif self.dtype == "bf16":
             t = t.view(_torch().int16)
         elif self.dtype in ("u16", "u32"):
             t = t.view({"u16": _torch().int16, "u32": _torch().int32}[self.dtype])
@@ -294,7 +303,7 @@ class Gpu:
             raise GpuError("wrap: need a contiguous tensor on this Gpu's device")
         if dtype is None:
             dtype = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16", torch.int8: "i8",
-                     torch.uint8: "u8", torch.int32: "i32", torch.int16: "i16"}[t.dtype]
+                     torch.uint8: "u8", torch.int32: "i32", torch.int16: "i16", torch.float8_e4m3fn: "f8"}[t.dtype]
         return Tensor(Buffer(t.data_ptr(), t.numel() * t.element_size(), owner=t), 0, tuple(t.shape), dtype)
 
     # -- native entry points ----------------------------------------------------------------------------------------
@@ -317,6 +326,32 @@ class Gpu:
         p = lambda t: t.ptr if t is not None else None  # noqa: E731
         self._check(lib().h3b_norm_mod_q8(self.ctx, x.ptr, x_stride, mod.ptr, mod_stride, rtype.ptr, out.ptr, p(sa), M, D,
                                            block, eps, int(ln), out_kind, p(y), p(post)))
+        if self._profile:
+            self.names.append(name)
+
+    def rms_f8_native(self, x: Tensor, x_stride: int, y: Tensor | None, y_stride: int, res: Tensor | None, res_stride: int,
+                      w: Tensor, out: Tensor, out_stride: int, sa: Tensor, sa_stride: int, M: int, D: int, eps: float,
+                      name: str = "rms_f8"):
+        self._check(lib().h3b_rms_f8(self.ctx, x.ptr, _ABI_DTYPE[x.dtype], x_stride, y.ptr if y is not None else None,
+                                      _ABI_DTYPE[y.dtype] if y is not None else 0, y_stride,
+                                      res.ptr if res is not None else None, res_stride, w.ptr, _ABI_DTYPE[w.dtype], out.ptr,
+                                      out_stride, sa.ptr, sa_stride, M, D, eps))
+        if self._profile:
+            self.names.append(name)
+
+    def quant_f8_native(self, x: Tensor, x_stride: int, out: Tensor, out_stride: int, sa: Tensor, sa_stride: int, M: int,
+                        D: int, mode: int, name: str = "quant_f8"):
+        self._check(lib().h3b_quant_f8(self.ctx, x.ptr, _ABI_DTYPE[x.dtype], x_stride, out.ptr, out_stride, sa.ptr,
+                                        sa_stride, M, D, mode))
+        if self._profile:
+            self.names.append(name)
+
+    def gemm_f8_native(self, a: Tensor, a_stride: int, sa: Tensor, sa_stride: int, w: Tensor, w_stride: int, sw: Tensor,
+                       sw_stride: int, bias: Tensor | None, out: Tensor, c_stride: int, M: int, N: int, K: int,
+                       name: str = "gemm(f8)"):
+        self._check(lib().h3b_gemm_f8(self.ctx, a.ptr, a_stride, sa.ptr, sa_stride, w.ptr, w_stride, sw.ptr, sw_stride,
+                                       bias.ptr if bias is not None else None, out.ptr, _ABI_DTYPE[out.dtype], c_stride, M,
+                                       N, K))
         if self._profile:
             self.names.append(name)
 

@@ -2,13 +2,14 @@
 the int8 product with its epilogue (h3metal/dit.py:209-217, h3metal/zimage.py:328-345: `ops.rot_q8` followed by
 `ops.gemm`). `QuantLinear` owns the layer's device buffers so that a step launches kernels and nothing else;
 `BlockLinears` strings the linears of one transformer block together for the benchmark and the smoke test.
+`BlockScaledLinear` is the layer in the e4m3 format with block scales.
 """
 
 from __future__ import annotations
 
 import numpy as np
 
-from . import ops, workloads
+from . import ops, quant, workloads
 from .gpu import Gpu, Tensor
 
 
@@ -42,6 +43,55 @@ def upload_weight(gpu: Gpu, codes, scales, bias=None, low=None) -> ops.QWeight:
         return gpu.upload(t) if isinstance(t, np.ndarray) else gpu.wrap(t)
     N, K = codes.shape
     return ops.QWeight("q8", put(codes), put(scales), int(N), int(K), bias=put(bias), low=low)
+
+
+def upload_weight_f8(gpu: Gpu, w: np.ndarray, bias=None) -> ops.QWeight:
+    """QWeight of format "f8" from a float weight [N][K] (and bias [N]): e4m3 codes, one scale per 128 x 128 block."""
+    codes, scales = quant.quant_f8(w)
+    N, K = w.shape
+    return ops.QWeight("f8", gpu.upload(codes, "f8"), gpu.upload(scales), int(N), int(K),
+                       bias=gpu.upload(np.ascontiguousarray(bias, dtype=np.float32)) if bias is not None else None)
+
+
+class BlockScaledLinear:
+    """y = x W^T (+ bias) with e4m3 codes and block scales on both sides, for up to M rows: the quantiser (plain rows, or
+    value | gate with swiglu_in) or, through normed(), the residual addition and RMSNorm in front of it, then the
+    product. Owns its buffers; a call may use fewer rows than M."""
+
+    def __init__(self, gpu: Gpu, wt: ops.QWeight, M: int, *, swiglu_in: bool = False, out_dtype: str = "bf16"):
+        self.gpu, self.wt, self.M, self.swiglu_in = gpu, wt, M, swiglu_in
+        self.codes = gpu.empty((M, quant.f8_stride(wt.K)), "f8")
+        self.sa = gpu.empty((-(-wt.K // quant.F8_GROUP), M), "f32")
+        self.out = gpu.empty((M, wt.N), out_dtype)
+
+    def _product(self, M: int) -> Tensor:
+        ops.gemm_f8(self.gpu, self.codes, self.wt, self.out, M, sa=self.sa, sa_stride=self.M)
+        return self.out
+
+    def _rows(self, M: int | None) -> int:
+        M = self.M if M is None else M
+        if not 0 < M <= self.M:
+            raise ValueError(f"{M} rows on a layer for up to {self.M}")
+        return M
+
+    def __call__(self, x: Tensor, M: int | None = None, *, x_stride: int | None = None) -> Tensor:
+        M = self._rows(M)
+        ops.quant_f8(self.gpu, x, self.codes, self.sa, M, self.wt.K, swiglu=self.swiglu_in, x_stride=x_stride,
+                     sa_stride=self.M)
+        return self._product(M)
+
+    def normed(self, x: Tensor, gain: Tensor, M: int | None = None, *, eps: float, y: Tensor | None = None,
+               res: Tensor | None = None) -> Tensor:
+        """The layer behind an RMSNorm: x (+ y, the sum kept in res or in x itself) is normed, coded and multiplied."""
+        if self.swiglu_in:
+            raise ValueError("normed: a layer behind a gated activation has no norm in front of it")
+        M = self._rows(M)
+        ops.rms_f8(self.gpu, x, gain, self.codes, self.sa, M, self.wt.K, eps=eps, y=y, res=res, sa_stride=self.M)
+        return self._product(M)
+
+    @property
+    def launches_per_call(self) -> int:
+        return 2
 
 
 class HostStaged:

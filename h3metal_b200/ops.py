@@ -7,6 +7,9 @@ function enqueues its kernels on `gpu`; results are available after `gpu.wait()`
 In scope: weight format "q8" with the storing epilogue (epi 0; outputs bf16 / f16 / f32) and the gated-residual
 epilogue (epi 1, with ksplit), with bias and with a low-rank (LoRA) term; `norm_mod_q8` (:200-211), the other producer of int8 activations. Other weight formats raise. `rot_q8` takes one argument the
 reference does not have, `block=` (the rotation block; the reference's kernel fixes it at 256).
+
+`rms_f8`, `quant_f8` and `gemm_f8` are the same layer in a second 8-bit format, which the reference does not have: e4m3
+codes with one fp32 scale per 128 channels, no rotation.
 """
 
 from __future__ import annotations
@@ -16,7 +19,7 @@ from dataclasses import dataclass, field, replace
 import numpy as np
 
 from .gpu import Gpu, Tensor, pack  # noqa: F401  (pack is re-exported like in the reference)
-from .quant import RB
+from .quant import F8_GROUP, RB, f8_stride
 
 FMT_ID = {"q8": 1, "q4": 2, "q4g": 3, "f16": 4, "bf16": 5, "h8": 6, "h4": 7, "h4g": 8}
 OUT_DT = {"f16": "half", "bf16": "bfloat", "f32": "float"}
@@ -24,10 +27,11 @@ OUT_DT = {"f16": "half", "bf16": "bfloat", "f32": "float"}
 
 @dataclass
 class QWeight:
-    """A linear layer's weight on the GPU: W[N][K], int8 codes with one fp32 scale per output row."""
-    fmt: str           # "q8" (the other formats of the reference are not part of this library)
-    w: Tensor          # codes, [N][K] row-major
-    sw: Tensor | None  # fp32 scales [N]
+    """A linear layer's weight on the GPU: W[N][K], int8 codes with one fp32 scale per output row, or e4m3 codes with one
+    per 128 x 128 block."""
+    fmt: str           # "q8", or "f8" for gemm_f8 (the other formats of the reference are not part of this library)
+    w: Tensor          # codes, [N][K] row-major ("f8": rows of quant.f8_stride(K) bytes)
+    sw: Tensor | None  # fp32 scales [N] ("f8": [ceil(N / 128)][ceil(K / 128)])
     N: int
     K: int
     G: int = 128
@@ -273,3 +277,82 @@ def rot_q8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor | None, M: int, D: int, 
         raise ValueError(f"rot_q8: {D} channels are not a multiple of the rotation block {block}")
     gpu.rot_q8_native(x, x_stride or (2 * D if swiglu else D), out, sa, M, D, block, 1 if swiglu else 0, out_hr,
                       name=f"rot_q8({D},b{block}{',swiglu' if swiglu else ''})")
+
+
+_FLOATS = ("bf16", "f16", "f32")
+
+
+def _rows(what: str, t: Tensor, types, rows: int, cols: int, stride: int):
+    """Refuses a tensor of another type, a stride shorter than its rows, and a buffer that ends before the last of them."""
+    if t.dtype not in types:
+        raise ValueError(f"{what}: type {t.dtype}, not {' / '.join(types)}")
+    if stride < cols or (rows - 1) * stride + cols > t.numel:
+        raise ValueError(f"{what}: {t.shape} does not hold {rows} rows of {cols} values {stride} apart")
+
+
+def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: int, *, eps: float, y: Tensor | None = None,
+           res: Tensor | None = None, x_stride: int | None = None, y_stride: int | None = None, res_stride: int | None = None,
+           out_stride: int | None = None, sa_stride: int | None = None):
+    """out, sa = e4m3 codes and scales of rmsnorm(x) * w (w [D], no offset). With y, first x + y, rounded to x's type and
+    kept in res (x itself by default), is what is normed. x, y and w are bf16, f16 or f32, each its own. out: "f8" rows of
+    quant.f8_stride(D) bytes; sa: fp32 [ceil(D / 128)][M], a group's scales of all rows side by side."""
+    if M <= 0 or D <= 0:
+        raise ValueError("rms_f8: M and D must be positive")
+    x_stride, out_stride, sa_stride = x_stride or D, out_stride or f8_stride(D), sa_stride or M
+    _rows("rms_f8 x", x, _FLOATS, M, D, x_stride)
+    _rows("rms_f8 w", w, _FLOATS, 1, D, D)
+    _rows("rms_f8 out", out, ("f8",), M, D, out_stride)
+    _rows("rms_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
+    if y is None:
+        if res is not None:
+            raise ValueError("rms_f8: res is where x + y goes: it needs y")
+        y_stride = res_stride = 0
+    else:
+        if res is None:
+            res, res_stride = x, res_stride or x_stride
+        y_stride, res_stride = y_stride or D, res_stride or D
+        _rows("rms_f8 y", y, _FLOATS, M, D, y_stride)
+        _rows("rms_f8 res", res, (x.dtype,), M, D, res_stride)
+    gpu.rms_f8_native(x, x_stride, y, y_stride, res, res_stride, w, out, out_stride, sa, sa_stride, M, D, eps,
+                      name=f"rms_f8({D}{',add' if y is not None else ''})" if gpu._profile else "")
+
+
+def quant_f8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor, M: int, D: int, *, swiglu: bool = False,
+             x_stride: int | None = None, out_stride: int | None = None, sa_stride: int | None = None):
+    """out, sa = e4m3 codes and scales of x (or of value * silu(gate) with the gates in columns D..2D-1); layouts as in
+    rms_f8."""
+    if M <= 0 or D <= 0:
+        raise ValueError("quant_f8: M and D must be positive")
+    wide = 2 * D if swiglu else D
+    x_stride, out_stride, sa_stride = x_stride or wide, out_stride or f8_stride(D), sa_stride or M
+    _rows("quant_f8 x", x, _FLOATS, M, wide, x_stride)
+    _rows("quant_f8 out", out, ("f8",), M, D, out_stride)
+    _rows("quant_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
+    gpu.quant_f8_native(x, x_stride, out, out_stride, sa, sa_stride, M, D, 1 if swiglu else 0,
+                        name=f"quant_f8({D}{',swiglu' if swiglu else ''})" if gpu._profile else "")
+
+
+def gemm_f8(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor, a_stride: int | None = None,
+            sa_stride: int | None = None, c_stride: int | None = None):
+    """out = A x W^T (+ bias) for e4m3 codes with block scales (a and sa as rms_f8 / quant_f8 leave them, wt of format
+    "f8"): fp32 sums, rounded once to out's type (bf16, f16 or f32). Exactly M rows are read and written."""
+    if wt.fmt != "f8":
+        raise ValueError(f"gemm_f8: weight format {wt.fmt!r}, not 'f8'")
+    if wt.low is not None:
+        raise NotImplementedError("gemm_f8: no low-rank term")
+    if wt.sw is None:
+        raise ValueError("gemm_f8: the weight has no block scales")
+    N, K = wt.N, wt.K
+    if M <= 0 or N <= 0 or K <= 0:
+        raise ValueError("gemm_f8: M, N and K must be positive")
+    groups = -(-K // F8_GROUP)
+    a_stride, sa_stride, c_stride, w_stride = a_stride or f8_stride(K), sa_stride or M, c_stride or N, wt.ws or f8_stride(K)
+    _rows("gemm_f8 a", a, ("f8",), M, K, a_stride)
+    _rows("gemm_f8 sa", sa, ("f32",), groups, M, sa_stride)
+    _rows("gemm_f8 weight", wt.w, ("f8",), N, K, w_stride)
+    _rows("gemm_f8 weight scales", wt.sw, ("f32",), -(-N // F8_GROUP), groups, groups)
+    _rows("gemm_f8 out", out, _FLOATS, M, N, c_stride)
+    if wt.bias is not None:
+        _rows("gemm_f8 bias", wt.bias, ("f32",), 1, N, N)
+    gpu.gemm_f8_native(a, a_stride, sa, sa_stride, wt.w, w_stride, wt.sw, groups, wt.bias, out, c_stride, M, N, K,
+                       name=f"gemm(f8,{K}->{N})" if gpu._profile else "")

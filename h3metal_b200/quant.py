@@ -81,13 +81,70 @@ def quant_q8(w: np.ndarray, search: bool = True):
     return codes, s.astype(np.float32)
 
 
+F8_GROUP = 128   # channels (and weight rows) that share a scale in the e4m3 format
+F8_TOP = 448.0   # largest finite e4m3 value
+_F8_TINY = 2.0 ** -126  # smallest scale: its reciprocal is still finite
+
+
+@functools.lru_cache(maxsize=1)
+def _e4m3_values() -> np.ndarray:
+    """The 127 non-negative finite e4m3 values in the order of their codes 0x00 .. 0x7E, fp64."""
+    code = np.arange(127)
+    exp, man = code >> 3, code & 7
+    return np.where(exp == 0, man * 2.0 ** -9, (8 + man) * 2.0 ** (exp - 10.0))
+
+
+def e4m3_bits(a: np.ndarray) -> np.ndarray:
+    """Values -> e4m3 codes (uint8), round to nearest even, saturating at +-448; NaN -> 0x7F."""
+    a = np.asarray(a, dtype=np.float64)
+    grid = _e4m3_values()
+    mag = np.minimum(np.where(np.isnan(a), 0.0, np.abs(a)), F8_TOP)
+    hi = np.clip(np.searchsorted(grid, mag), 1, 126)
+    below, above = mag - grid[hi - 1], grid[hi] - mag
+    code = np.where((above < below) | ((above == below) & (hi % 2 == 0)), hi, hi - 1).astype(np.uint8)
+    return np.where(np.isnan(a), np.uint8(0x7F), code | (np.signbit(a).astype(np.uint8) << 7)).astype(np.uint8)
+
+
+def e4m3_to_f32(u: np.ndarray) -> np.ndarray:
+    """e4m3 codes (uint8) -> fp32."""
+    u = np.asarray(u, dtype=np.uint8)
+    table = np.append(_e4m3_values(), np.nan).astype(np.float32)
+    return np.where(u & 0x80, -table[u & 0x7F], table[u & 0x7F])
+
+
+def f8_stride(k: int) -> int:
+    """Row stride of e4m3 codes of k channels: whole 16-byte pieces."""
+    return -(-k // 16) * 16
+
+
+def quant_f8(w: np.ndarray):
+    """Weight [N][K] -> (e4m3 codes uint8 [N][f8_stride(K)], fp32 scales [ceil(N / 128)][ceil(K / 128)]): one scale per
+    128 x 128 block, its largest magnitude / 448 (1 for a block of zeros). Bytes past K are zero."""
+    n, k = w.shape
+    rows, cols = -(-n // F8_GROUP), -(-k // F8_GROUP)
+    codes = np.zeros((n, f8_stride(k)), np.uint8)
+    scales = np.ones((rows, cols), np.float32)
+    for i in range(rows):
+        band = w[i * F8_GROUP:(i + 1) * F8_GROUP].astype(np.float32)
+        full = np.zeros((len(band), cols * F8_GROUP), np.float32)
+        full[:, :k] = band
+        blocks = full.reshape(len(band), cols, F8_GROUP)
+        top = np.abs(blocks).max(axis=(0, 2))
+        scales[i] = np.where(top > 0, np.maximum(top / np.float32(F8_TOP), np.float32(_F8_TINY)), np.float32(1.0))
+        codes[i * F8_GROUP:(i + 1) * F8_GROUP, :k] = e4m3_bits(blocks / scales[i][None, :, None]).reshape(len(band), -1)[:, :k]
+    return codes, scales
+
+
 _INT8_FORMATS = ("q8", "h8")
 
 
 def dequant(fmt: str, w: np.ndarray, sw: np.ndarray | None, N: int, K: int, G: int = 128) -> np.ndarray:
-    """The fp32 matrix [N][K] stored codes stand for (in the rotated input space). int8 and bf16/f16 only."""
+    """The fp32 matrix [N][K] stored codes stand for (int8: in the rotated input space). int8, e4m3 and bf16/f16 only."""
     if fmt in _INT8_FORMATS:
         return w.astype(np.float32) * sw[:, None]
+    if fmt == "f8":
+        spread = np.repeat(np.repeat(sw, F8_GROUP, axis=0)[:N], F8_GROUP, axis=1)[:, :K]
+        return e4m3_to_f32(w[:, :K]) * spread
     if fmt == "f16":
         return w.astype(np.float32)
     if fmt == "bf16":
@@ -96,9 +153,11 @@ def dequant(fmt: str, w: np.ndarray, sw: np.ndarray | None, N: int, K: int, G: i
 
 
 def quantize(fmt: str, w: np.ndarray, G: int = 128):
-    """-> (stored codes, scales or None) for the formats this package carries (q8/h8, f16, bf16)."""
+    """-> (stored codes, scales or None) for the formats this package carries (q8/h8, f8, f16, bf16)."""
     if fmt in _INT8_FORMATS:
         return quant_q8(w)
+    if fmt == "f8":
+        return quant_f8(w)
     if fmt == "f16":
         return w.astype(np.float16), None
     if fmt == "bf16":

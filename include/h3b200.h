@@ -33,7 +33,7 @@ extern "C" {
 typedef struct h3b_ctx h3b_ctx;
 
 /* element types of tensor arguments */
-enum { H3B_F32 = 0, H3B_F16 = 1, H3B_BF16 = 2, H3B_I8 = 3, H3B_I32 = 4 };
+enum { H3B_F32 = 0, H3B_F16 = 1, H3B_BF16 = 2, H3B_I8 = 3, H3B_I32 = 4, H3B_F8 = 5 /* e4m3 */ };
 
 /* Message of the last failed call on this thread (empty if none). Replaces h3_last_error (src/capi.h:27). */
 H3B_API const char *h3b_last_error(void);
@@ -288,6 +288,32 @@ H3B_API int h3b_gemm_set_store_mode(h3b_ctx *ctx, int mode);
  * TMA-fed kernel owns, 32 or 64 (0 = automatic). The counterpart of the NSG/MAXB geometry of
  * h3metal/ops.py:193-197. Returns 0. */
 H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages, int chunk);
+
+/* ---- Block-scaled e4m3 linear layers -------------------------------------------------------------------------------
+ * The second 8-bit number format beside int8: e4m3 codes with one fp32 scale per 128 channels of a row (activations)
+ * or per 128 x 128 block (weights), without a rotation. No counterpart in the reference. For rows v[m][D]:
+ *   s[g][m] = max(max_{k in group g} |v[m][k]| / 448, 2^-126), 1 where the group is all zero; code = e4m3(v / s),
+ *   nearest, ties to even. G = ceil(D / 128) groups; a last group of D % 128 channels has a scale of its own.
+ * Codes are bytes [M][out_stride] (rows 16-byte aligned; bytes past D are not written), scales fp32
+ * [G][sa_stride >= M]: a group's scales of all rows side by side. Any M, N, D, K >= 1. A NaN stays a NaN in its own
+ * place; a group that holds an infinity reads back as NaN. Rows past M are neither read nor written.
+ *
+ *   h3b_rms_f8    h = x (+ y);  v = h / sqrt(mean(h^2) + eps) * w.   x [M][x_stride], w [D]; with y [M][y_stride] the sum h
+ *                 is rounded to x's type, stored to res [M][res_stride] (x's type; res may be x) and then normed;
+ *                 without y, res must be NULL. x, y, w of type bf16, f16 or f32 each. D <= 32768.
+ *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D])
+ *   h3b_gemm_f8   C[m][n] = c_dtype(sum_g sa[g][m] * sw[n / 128][g] * sum_{k in g} A[m][k] * W[n][k]  (+ bias[n]))
+ *                 A codes [M][a_stride], W codes [N][w_stride] (K-contiguous, rows 16-byte aligned), sa as above,
+ *                 sw fp32 [ceil(N / 128)][sw_stride >= G], bias fp32 [N] or NULL, C [M][c_stride] bf16, f16 or f32.
+ *                 Sums are fp32; the result does not vary from call to call. */
+H3B_API int h3b_rms_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, const void *y, int y_dtype,
+                       int64_t y_stride, void *res, int64_t res_stride, const void *w, int w_dtype, void *out,
+                       int64_t out_stride, float *sa, int64_t sa_stride, int M, int D, float eps);
+H3B_API int h3b_quant_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, void *out, int64_t out_stride,
+                         float *sa, int64_t sa_stride, int M, int D, int mode);
+H3B_API int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, int64_t sa_stride, const void *W,
+                        int64_t w_stride, const float *sw, int64_t sw_stride, const float *bias, void *C, int c_dtype,
+                        int64_t c_stride, int M, int N, int K);
 
 /* Self-test of the error path the kernels share. Every device-side wait in this library is bounded: when one runs
  * out the kernel records a code in the context's status word, winds down and returns, and the next h3b_wait reports
