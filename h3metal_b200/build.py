@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libh3b200.so")
 SOURCES = ("capi.cu", "rot_q8.cu", "rot_q8_tma.cu", "norm_mod_q8.cu", "gemm_w8a8.cu", "gemm_w8a8_pair.cu", "dequant.cu", "peer.cu", "mma_probe.cu",
-           "rows_f8.cu", "gemm_f8_small.cu")
+           "rows_f8.cu", "gemm_f8_small.cu", "gemm_f8_pair.cu")
 HEADERS = ("kernels.h", "ptx.cuh", "rot_common.cuh", "gemm_common.cuh", os.path.join("..", "..", "include", "h3b200.h"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # -fmad=false: the rotate+quantise arithmetic and the dequantising epilogue are defined operation by operation;

@@ -86,6 +86,7 @@ struct h3b_ctx {
   int overlap = 1;  // programmatic dependent launch of the path's main kernels (h3b_set_launch_overlap); on by default
   int pair_stages = 0, pair_clusters = 0;  // CTA-pair product: ring depth and resident clusters (0 = unavailable)
   int pair_stages_staged = 0;              // ring depth when 64 KB of shared memory stage the outputs for TMA stores
+  int f8_pair_clusters = 0;                // the same for the block-scaled product
   int store_mode = 0;                      // staged (TMA) stores of the pair product: 0 automatic, 1 whenever possible, -1 never
   uint64_t launches = 0;
   std::string name;
@@ -276,6 +277,7 @@ h3b_ctx *h3b_open(int device) {
   if ((e = h3b::gemm_configure(device)) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
   if ((e = h3b::gemm_pair_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
   if ((e = h3b::gemm_f8_small_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
+  if ((e = h3b::gemm_f8_pair_configure(&ctx->f8_pair_clusters)) != cudaSuccess) return bail("gemm_f8 set-up", e);
   ctx->pair_stages = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, false);
   ctx->pair_stages_staged = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, true);
   ctx->pair_clusters = ctx->pair_stages >= 2 ? h3b::gemm_pair_max_clusters(ctx->pair_stages) : 0;
@@ -900,13 +902,37 @@ int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, 
   memset(&g, 0, sizeof g);
   g.sa = sa; g.sw = sw; g.bias = bias; g.c = C; g.c_stride = c_stride; g.sa_stride = sa_stride; g.sw_stride = sw_stride;
   g.c_dtype = c_dtype; g.M = M; g.N = N; g.K = K;
+  g.overlap = (ctx->overlap != 0 && !ctx->profile) ? 1 : 0;
+  g.status = ctx->status_dev;
+  const bool pair = M > 128 && N > 128 && ctx->f8_pair_clusters > 0;
+  const CUtensorMap *m;
+  if (pair) {
+    g.m_tiles = (M - 1) / 256 + 1;
+    const long long tiles = static_cast<long long>(g.m_tiles) * ((N - 1) / 256 + 1);
+    if (tiles > 0x3FFFFFFFLL) return fail("gemm_f8: too many tiles for one launch");
+    // a band of A rows (32 MB) stays in L2 while W streams through once per band, as in the int8 product
+    long long band = (32LL << 20) / (256LL * K);
+    if (band < 2) band = 2;
+    g.band = static_cast<int>(band < g.m_tiles ? band : g.m_tiles);
+    if (!(m = ctx->tensor_map(A, h3b::kDtypeI8, K, M, a_stride, 128, 128, 128))) return -1;
+    g.map_a = *m;
+    if (!(m = ctx->tensor_map(W, h3b::kDtypeI8, K, N, w_stride, 128, 128, 128))) return -1;
+    g.map_w = *m;
+    // TMA cuts a row off at whole 16-byte pieces: with another N it would write past the last column
+    if (c_dtype != H3B_F32 && rows_aligned(C, c_stride, 2) && N % 8 == 0) {
+      if (!(m = ctx->tensor_map(C, c_dtype, N, M, c_stride * 2, 64, 32, 128))) return -1;
+      g.map_c = *m;
+      g.tma_store = 1;
+    }
+    cudaEvent_t ps = nullptr;
+    if (ctx->before_launch(&ps)) return -1;
+    const int clusters = static_cast<int>(tiles < ctx->f8_pair_clusters ? tiles : ctx->f8_pair_clusters);
+    return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_pair(g, clusters, ctx->stream));
+  }
   g.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   g.m_tiles = (M - 1) / g.nt + 1;
   g.split = 1;
-  g.overlap = (ctx->overlap != 0 && !ctx->profile) ? 1 : 0;
-  g.status = ctx->status_dev;
   if (((N - 1LL) / 128 + 1) * g.m_tiles * g.split > 0x7FFFFFFFLL) return fail("gemm_f8: too many tiles for one launch");
-  const CUtensorMap *m;
   if (!(m = ctx->tensor_map(A, h3b::kDtypeI8, K, M, a_stride, 128, g.nt, 128))) return -1;
   g.map_a = *m;
   if (!(m = ctx->tensor_map(W, h3b::kDtypeI8, K, N, w_stride, 128, 128, 128))) return -1;

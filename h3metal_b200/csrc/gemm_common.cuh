@@ -123,6 +123,21 @@ __device__ __forceinline__ void store_segment(OUT_T *dst, const float (&v)[32], 
   }
 }
 
+constexpr int kOutPanel = 32 * 128;  // staged stores: 32 rows x 64 two-byte columns
+
+// 32 consecutive output values of row `lane` of the warp, packed to 16-bit, into the warp's staging panel that
+// holds columns [64 * (c / 2), +64): piece p of row r sits at p ^ (r & 7) (the 128-byte swizzle TMA expects).
+template <typename OUT_T>
+__device__ __forceinline__ void stage_out32(uint8_t *warp_buf, int c, int lane, const float (&v)[32]) {
+  uint32_t w[32];
+  Packed<OUT_T>::pack(v, w);
+  uint8_t *row = warp_buf + (c >> 1) * kOutPanel + lane * 128;
+  const int first = (c & 1) * 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4 *>(row + (((first + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
 // float(acc) * sa * sw (+ bias) (+ low) for 32 columns, two at a time with the packed fp32 instructions (each half is
 // rounded exactly like the scalar operation): convert, times the row scale, times the column scale, plus bias,
 // plus the low-rank term.

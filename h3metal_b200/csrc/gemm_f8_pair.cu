@@ -1,0 +1,320 @@
+// Block-scaled e4m3 product on CTA pairs: C tile 256 x 256 per cluster of two CTAs, tcgen05.mma cta_group::2.
+//
+//   C[m][n] = sum_g sa[g][m] * sw[n / 128][g] * P_g[m][n] (+ bias[n]),   P_g = the group's 128 channels of A W^T
+//
+// As in gemm_f8_small.cu a group's P_g (four instructions of 32 channels, fp32 in tensor memory) is added, scaled, to
+// running sums in fp32 registers. An epilogue thread owns one row of the tile and 128 of its columns - exactly the columns
+// of one weight block, so that the scale of a group is ONE number per thread, sa * sw - and 128 running sums.
+//
+// What bounds it: the tensor cores, 512 cycles per group and SM, if the epilogue keeps up. Reading a group out of tensor
+// memory takes 256 cycles per SM and its 128 x 256 multiply-adds as many (two columns per instruction, packed fp32); two
+// accumulators of 256 columns let the MMAs of a group run while the group before is read.
+//
+// Roles per CTA (rank 0 = leader): warp 0 TMA producer (own 128 rows of A, own half of the 256 rows of W per group, bytes
+// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..11
+// epilogue: four lane quarters x two column halves; the first four warps hand them most of their registers. 16-bit results are staged in shared memory as 128-byte-swizzled panels and stored by TMA
+// while the next tile runs; fp32 results and unaligned outputs are stored from registers. Set-up overlaps the kernel before
+// (programmatic stream serialization). All waits are bounded. No load uses multicast.
+#include <cuda.h>
+
+#include "gemm_common.cuh"
+
+namespace h3b {
+namespace {
+
+using namespace gemm;
+
+constexpr int kF8BN = 256;
+constexpr int kF8Stage = kABytes + 128 * kBKBytes;  // 32 KB: this CTA's rows of A and its half of W
+constexpr int kF8EpiWarps = 8;
+constexpr int kF8Threads = 128 + 32 * kF8EpiWarps;
+// Registers per thread after the split: 128 x 56 + 256 x 224 = 64512 = 384 x 168, what the launch was given.
+constexpr int kF8RegsIssue = 56, kF8RegsEpi = 224;
+constexpr int kF8OutWarp = 2 * kOutPanel;           // a warp's 32 rows x 128 two-byte columns
+constexpr int kF8OutBytes = kF8EpiWarps * kF8OutWarp;
+
+// acc += p * s for sixteen columns, two at a time
+__device__ __forceinline__ void scale_add16(const uint32_t (&p)[16], float2 s2, float2 *acc) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    acc[j] = __ffma2_rn(make_float2(__uint_as_float(p[2 * j]), __uint_as_float(p[2 * j + 1])), s2, acc[j]);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
+gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t *base_ptr = smem_raw + (base - raw_addr);
+  // [ring: stages x 32 KB][staged stores: 64 KB, optional][barriers 256 B]
+  const uint32_t out_off = stages * kF8Stage;
+  const uint32_t bars_off = out_off + (g.tma_store ? kF8OutBytes : 0);
+  const uint32_t bars = base + bars_off;
+  auto full_bar = [&](int i) { return bars + 8u * i; };
+  auto empty_bar = [&](int i) { return bars + 64u + 8u * i; };
+  auto acc_full_bar = [&](int i) { return bars + 128u + 8u * i; };
+  auto acc_empty_bar = [&](int i) { return bars + 144u + 8u * i; };
+  volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(base_ptr + bars_off + 176);
+  volatile int *cta_abort = reinterpret_cast<volatile int *>(base_ptr + bars_off + 180);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_cta_rank();
+  const bool leader = rank == 0;
+  const int n_tiles = (g.N + kF8BN - 1) / kF8BN;
+  const int num_tiles = g.m_tiles * n_tiles;
+  const int groups = (g.K + kBKBytes - 1) / kBKBytes;
+  const int first_tile = cluster_id_x(), tile_step = cluster_count_x();
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_descriptor(&g.map_a);
+    tma_prefetch_descriptor(&g.map_w);
+    if (g.tma_store) tma_prefetch_descriptor(&g.map_c);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(full_bar(i), 1);   // the leader's producer arms it; bytes arrive from both CTAs
+      mbar_init(empty_bar(i), 1);  // one commit arrival per use
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full_bar(i), 1);
+      mbar_init(acc_empty_bar(i), 2 * kF8EpiWarps);
+    }
+    *cta_abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(const_cast<uint32_t *>(tmem_holder)), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  grid_dep_launch();
+  grid_dep_wait();  // global memory is read and written from here on only
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8RegsIssue));
+    if (warp == 0) {
+      if (lane == 0) {
+        RingPos pos;
+        uint32_t filled = 0;  // stages filled so far, saturating at `stages` (for the wind-down)
+        const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
+        bool ok = true;
+        for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+          const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
+          const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128;
+          const int n0 = tc.n_blk * kF8BN + static_cast<int>(rank) * 128;
+          for (int kb = 0; kb < groups; ++kb) {
+            const uint32_t s = pos.s;
+            ok = mbar_wait(empty_bar(s), pos.ph ^ 1u, cta_abort, g.status, kStatusProducerTimeout);
+            if (!ok) break;
+            if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * kF8Stage);
+            const uint32_t leader_full = leader_full0 + 8u * s;
+            const uint32_t dst = base + s * kF8Stage;
+            tma_load_2d_pair(dst, &g.map_a, leader_full, kb * kBKBytes, m0);
+            tma_load_2d_pair(dst + kABytes, &g.map_w, leader_full, kb * kBKBytes, n0);
+            pos.advance(stages);
+            filled += filled < static_cast<uint32_t>(stages);
+          }
+        }
+        if (*cta_abort && leader) {
+          // wind-down after a timeout: the pair's copies into the last stages filled are counted on the leader's full
+          // barriers; wait (bounded) for them so that neither CTA leaves with copies still landing in its shared memory
+          for (uint32_t j = 0; j < filled; ++j) {
+            pos.retreat(stages);
+            int dummy_abort = 0;
+            mbar_wait(full_bar(pos.s), pos.ph, &dummy_abort, g.status, kStatusDrainTimeout, kDrainLimitCycles);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (leader && lane == 0) {
+        constexpr uint32_t idesc = umma_instr_desc(1, 0, 256, kF8BN);  // f32 accumulate, e4m3 x e4m3, M 256 over the pair
+        const uint64_t ad0 = umma_smem_desc(base, 1024, 2);
+        const uint64_t bd0 = umma_smem_desc(base + kABytes, 1024, 2);
+        RingPos pos, buf;
+        bool ok = true;
+        for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+          for (int kb = 0; kb < groups; ++kb) {
+            ok = mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout);
+            if (!ok) break;
+            const uint32_t s = pos.s;
+            ok = mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint64_t ad = ad0 + static_cast<uint64_t>(s * (kF8Stage >> 4));
+            const uint64_t bd = bd0 + static_cast<uint64_t>(s * (kF8Stage >> 4));
+            const uint32_t d = tmem_base + buf.s * kF8BN;
+#pragma unroll
+            for (int k = 0; k < kBKBytes / 32; ++k) umma_f8_pair(d, ad + 2u * k, bd + 2u * k, idesc, k ? 1u : 0u);
+            umma_commit_pair(empty_bar(s), 3);
+            umma_commit_pair(acc_full_bar(buf.s), 3);
+            pos.advance(stages);
+            buf.advance(2);
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8RegsEpi));
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int row = quarter * 32 + lane;
+    const bool staged = g.tma_store != 0;
+    uint8_t *out_buf = base_ptr + out_off + (half * 4 + quarter) * kF8OutWarp;
+    const uint32_t out_addr = base + out_off + (half * 4 + quarter) * kF8OutWarp;
+    const size_t esize = g.c_dtype == kDtypeF32 ? 4 : 2;
+    const bool vec_ok = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && (g.c_stride * esize) % 16 == 0;
+    const int n_blocks = (g.N + 127) / 128;
+    const uint32_t leader_acc_empty0 = map_to_cta(acc_empty_bar(0), 0);
+    RingPos buf;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
+      const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
+      const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128, n0 = tc.n_blk * kF8BN + half * 128;
+      const int m = m0 + row;
+      // rows and columns past the end compute zeros (TMA fills their codes with them) and are not stored: any scale will do
+      const float *sa_p = g.sa + min(m, g.M - 1);
+      const float *sw_p = g.sw + static_cast<size_t>(min(n0 / 128, n_blocks - 1)) * g.sw_stride;
+      float bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + j * 32 + lane;
+        bias[j] = g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
+      }
+      float2 acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+      // scales two groups ahead of their use
+      float a0 = __ldg(sa_p), w0 = __ldg(sw_p), a1 = 0.0f, w1 = 0.0f;
+      if (groups > 1) {
+        a1 = __ldg(sa_p + g.sa_stride);
+        w1 = __ldg(sw_p + 1);
+      }
+      for (int kb = 0; kb < groups; ++kb) {
+        const float s = __fmul_rn(a0, w0);
+        a0 = a1; w0 = w1;
+        if (kb + 2 < groups) {
+          a1 = __ldg(sa_p + static_cast<size_t>(kb + 2) * g.sa_stride);
+          w1 = __ldg(sw_p + kb + 2);
+        }
+        ok = mbar_wait(acc_full_bar(buf.s), buf.ph, cta_abort, g.status, kStatusEpilogueTimeout);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {  // a warp gives up as a whole
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * kF8BN + half * 128;
+        const float2 s2 = make_float2(s, s);
+        // two register sets: the next sixteen columns are on their way while these are added
+        uint32_t p[2][16];
+        tmem_ld_32x32b_x16(t_acc, p[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_ld_wait();
+          if (c < 7) {
+            tmem_ld_32x32b_x16(t_acc + (c + 1) * 16, p[(c + 1) & 1]);
+          } else {  // the warp's last values of the group are in registers: the leader may overwrite them
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8u * buf.s);
+          }
+          scale_add16(p[c & 1], s2, acc + c * 8);
+        }
+        buf.advance(2);
+      }
+      if (!ok) break;
+      if (staged) {  // the panels of the tile before must have been read out of shared memory
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[2 * j] = acc[c * 16 + j].x;
+          v[2 * j + 1] = acc[c * 16 + j].y;
+        }
+        if (g.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], __shfl_sync(0xFFFFFFFFu, bias[c], j));
+        }
+        if (staged) {
+          if (g.c_dtype == kDtypeBf16) stage_out32<__nv_bfloat16>(out_buf, c, lane, v);
+          else stage_out32<__half>(out_buf, c, lane, v);
+        } else {
+          const int n = n0 + c * 32, n_valid = g.N - n;
+          if (m < g.M && n_valid > 0) {
+            const size_t at = static_cast<size_t>(m) * g.c_stride + n;
+            if (g.c_dtype == kDtypeF32) store_segment(static_cast<float *>(g.c) + at, v, n_valid, vec_ok);
+            else if (g.c_dtype == kDtypeBf16) store_segment(static_cast<__nv_bfloat16 *>(g.c) + at, v, n_valid, vec_ok);
+            else store_segment(static_cast<__half *>(g.c) + at, v, n_valid, vec_ok);
+          }
+        }
+      }
+      if (staged) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int y = m0 + quarter * 32;
+          if (y < g.M) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (n0 + i * 64 < g.N) tma_store_2d(&g.map_c, out_addr + i * kOutPanel, n0 + i * 64, y);
+          }
+          tma_store_commit();
+        }
+      }
+    }
+    if (staged && lane == 0) tma_store_wait_all();
+    __syncwarp();
+  }
+
+  // Neither CTA may leave while the other can still read its shared memory, signal its barriers or write its TMEM.
+  tc_fence_before_sync();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+size_t pair_bytes(int stages, bool staged) {
+  return 1024 + static_cast<size_t>(stages) * kF8Stage + (staged ? kF8OutBytes : 0) + kBarrierBytes;
+}
+int pair_stages(bool staged) { return staged ? 5 : 6; }
+
+}  // namespace
+
+cudaError_t gemm_f8_pair_configure(int *clusters) {
+  static_assert(1024 + 5 * kF8Stage + kF8OutBytes + kBarrierBytes <= 232448, "ring and staging share 227 KB");
+  *clusters = 0;
+  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(kF8Threads, 1, 1);
+  cfg.dynamicSmemBytes = pair_bytes(pair_stages(true), true);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(clusters, gemm_f8_pair_kernel, &cfg);
+}
+
+cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
+  const bool staged = g.tma_store != 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * clusters);  // the cluster shape (2, 1, 1) is part of the kernel's declaration
+  cfg.blockDim = dim3(kF8Threads);
+  cfg.dynamicSmemBytes = pair_bytes(pair_stages(staged), staged);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g.overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel, g, pair_stages(staged));
+}
+
+}  // namespace h3b

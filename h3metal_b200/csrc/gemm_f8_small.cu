@@ -175,7 +175,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
       const float ws_next = kb + 1 < g_end ? __ldg(sw_row + kb + 1) : 0.0f;
       cp_async_wait<kScaleSlots - 1>();
       __syncwarp();
-      if (!mbar_wait(acc_full_bar(buf.s), buf.ph, cta_abort, g.status, kStatusEpilogueTimeout)) break;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(acc_full_bar(buf.s), buf.ph, cta_abort, g.status, kStatusEpilogueTimeout))) break;
       tc_fence_after_sync();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * NT;
       const float *s4 = my_scales + (kb & (kScaleSlots - 1)) * NT;

@@ -45,22 +45,8 @@ constexpr int kHalfWBytes = 128 * kBKBytes;        // this CTA's half of the W t
 constexpr int kPairStage = kABytes + kHalfWBytes;  // 32 KB
 constexpr int kPairMaxStages = 6;
 constexpr int kHalfBBytes = 128 * kLoraChunk * 2;  // this CTA's half of a 32-rank chunk of B': 8 KB
-constexpr int kOutPanel = 32 * 128;                // 32 rows x 64 two-byte columns
 constexpr int kOutWarp = 4 * kOutPanel;            // a warp's 32 rows x 256 columns
 constexpr int kOutBytes = 4 * kOutWarp;            // 64 KB per CTA
-
-// 32 consecutive output values of row `lane` of the warp, packed to 16-bit, into the warp's staging panel that
-// holds columns [64 * (c / 2), +64): piece p of row r sits at p ^ (r & 7) (the 128-byte swizzle TMA expects).
-template <typename OUT_T>
-__device__ __forceinline__ void stage_out32(uint8_t *warp_buf, int c, int lane, const float (&v)[32]) {
-  uint32_t w[32];
-  Packed<OUT_T>::pack(v, w);
-  uint8_t *row = warp_buf + (c >> 1) * kOutPanel + lane * 128;
-  const int first = (c & 1) * 4;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint4 *>(row + (((first + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-}
 
 template <bool LORA, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EPI, 1)

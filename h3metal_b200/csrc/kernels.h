@@ -187,17 +187,23 @@ constexpr int kRmsF8MaxD = 32768;
 cudaError_t launch_rms_f8(const RmsF8Launch &r, bool overlap, cudaStream_t stream);
 
 struct GemmF8Launch {
-  CUtensorMap map_a;   // e4m3 [M][K], box nt x 128 bytes, 128-byte swizzle
+  CUtensorMap map_a;   // e4m3 [M][K], box nt x 128 bytes (pairs: 128 x 128), 128-byte swizzle
   CUtensorMap map_w;   // e4m3 [N][K], box 128 x 128 bytes
+  CUtensorMap map_c;   // 16-bit output [M][N], box 32 rows x 64 columns, 128-byte swizzle (tma_store only)
   const float *sa, *sw, *bias;
   void *c;
   long long c_stride, sa_stride, sw_stride;
   int c_dtype, M, N, K;
-  int nt, m_tiles, split;  // rows of A per tile, tiles of that height, CTAs that share K
+  int m_tiles;         // tiles of nt (pairs: 256) rows
+  int nt, split;       // few rows: rows of A per tile, CTAs that share K
+  int band, tma_store; // pairs: row tiles swept per column tile; 16-bit results staged and stored by TMA
   int overlap;
   int *status;
 };
 cudaError_t gemm_f8_small_configure();
 cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, cudaStream_t stream);
+// CTA pairs on 256 x 256 tiles; *clusters: pairs that can be resident at once
+cudaError_t gemm_f8_pair_configure(int *clusters);
+cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream);
 
 }  // namespace h3b
