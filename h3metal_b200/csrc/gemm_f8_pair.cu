@@ -11,8 +11,8 @@
 // accumulators of 256 columns let the MMAs of a group run while the group before is read.
 //
 // Roles per CTA (rank 0 = leader): warp 0 TMA producer (own 128 rows of A, own half of the 256 rows of W per group, bytes
-// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..11
-// epilogue: four lane quarters x two column halves; the first four warps hand them most of their registers. 16-bit results are staged in shared memory as 128-byte-swizzled panels and stored by TMA
+// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..19
+// epilogue: four lane quarters x four parts of 64 columns; the first four warps hand them most of their registers. 16-bit results are staged in shared memory as 128-byte-swizzled panels and stored by TMA
 // while the next tile runs; fp32 results and unaligned outputs are stored from registers. Set-up overlaps the kernel before
 // (programmatic stream serialization). All waits are bounded. No load uses multicast.
 #include <cuda.h>
@@ -26,17 +26,19 @@ using namespace gemm;
 
 constexpr int kF8BN = 256;
 constexpr int kF8Stage = kABytes + 128 * kBKBytes;  // 32 KB: this CTA's rows of A and its half of W
-constexpr int kF8EpiWarps = 8;
+constexpr int kF8EpiWarps = 16;
+constexpr int kF8Cols = kF8BN / (kF8EpiWarps / 4);  // columns per epilogue thread
+static_assert(kF8Cols == 64, "a warp's columns are one staging panel and lie in one weight block");
 constexpr int kF8Threads = 128 + 32 * kF8EpiWarps;
-// Registers per thread after the split: 128 x 56 + 256 x 224 = 64512 = 384 x 168, what the launch was given.
-constexpr int kF8RegsIssue = 56, kF8RegsEpi = 224;
-constexpr int kF8OutWarp = 2 * kOutPanel;           // a warp's 32 rows x 128 two-byte columns
+// Registers per thread after the split: 128 x 32 + 512 x 112 = 61440 = 640 x 96, what the launch was given.
+constexpr int kF8RegsIssue = 32, kF8RegsEpi = 112;
+constexpr int kF8OutWarp = kOutPanel;               // a warp's 32 rows x 64 two-byte columns
 constexpr int kF8OutBytes = kF8EpiWarps * kF8OutWarp;
 
-// acc += p * s for sixteen columns, two at a time
-__device__ __forceinline__ void scale_add16(const uint32_t (&p)[16], float2 s2, float2 *acc) {
+// acc += p * s for 32 columns, two at a time
+__device__ __forceinline__ void scale_add32(const uint32_t (&p)[32], float2 s2, float2 *acc) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 16; ++j)
     acc[j] = __ffma2_rn(make_float2(__uint_as_float(p[2 * j]), __uint_as_float(p[2 * j + 1])), s2, acc[j]);
 }
 
@@ -51,8 +53,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
   const uint32_t bars_off = out_off + (g.tma_store ? kF8OutBytes : 0);
   const uint32_t bars = base + bars_off;
   auto full_bar = [&](int i) { return bars + 8u * i; };
-  auto empty_bar = [&](int i) { return bars + 64u + 8u * i; };
-  auto acc_full_bar = [&](int i) { return bars + 128u + 8u * i; };
+  auto done_bar = [&](int i) { return bars + 64u + 8u * i; };
   auto acc_empty_bar = [&](int i) { return bars + 144u + 8u * i; };
   volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(base_ptr + bars_off + 176);
   volatile int *cta_abort = reinterpret_cast<volatile int *>(base_ptr + bars_off + 180);
@@ -70,13 +71,10 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
     tma_prefetch_descriptor(&g.map_w);
     if (g.tma_store) tma_prefetch_descriptor(&g.map_c);
     for (int i = 0; i < stages; ++i) {
-      mbar_init(full_bar(i), 1);   // the leader's producer arms it; bytes arrive from both CTAs
-      mbar_init(empty_bar(i), 1);  // one commit arrival per use
+      mbar_init(full_bar(i), 1);  // the leader's producer arms it; bytes arrive from both CTAs
+      mbar_init(done_bar(i), 1);  // one commit arrival per use
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(acc_full_bar(i), 1);
-      mbar_init(acc_empty_bar(i), 2 * kF8EpiWarps);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(acc_empty_bar(i), 2 * kF8EpiWarps);
     *cta_abort = 0;
     fence_barrier_init();
   }
@@ -105,7 +103,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
           const int n0 = tc.n_blk * kF8BN + static_cast<int>(rank) * 128;
           for (int kb = 0; kb < groups; ++kb) {
             const uint32_t s = pos.s;
-            ok = mbar_wait(empty_bar(s), pos.ph ^ 1u, cta_abort, g.status, kStatusProducerTimeout);
+            ok = mbar_wait(done_bar(s), pos.ph ^ 1u, cta_abort, g.status, kStatusProducerTimeout);
             if (!ok) break;
             if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * kF8Stage);
             const uint32_t leader_full = leader_full0 + 8u * s;
@@ -146,8 +144,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
             const uint32_t d = tmem_base + buf.s * kF8BN;
 #pragma unroll
             for (int k = 0; k < kBKBytes / 32; ++k) umma_f8_pair(d, ad + 2u * k, bd + 2u * k, idesc, k ? 1u : 0u);
-            umma_commit_pair(empty_bar(s), 3);
-            umma_commit_pair(acc_full_bar(buf.s), 3);
+            umma_commit_pair(done_bar(s), 3);  // the stage may be refilled, the accumulator read
             pos.advance(stages);
             buf.advance(2);
           }
@@ -156,33 +153,33 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8RegsEpi));
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
     const int row = quarter * 32 + lane;
     const bool staged = g.tma_store != 0;
-    uint8_t *out_buf = base_ptr + out_off + (half * 4 + quarter) * kF8OutWarp;
-    const uint32_t out_addr = base + out_off + (half * 4 + quarter) * kF8OutWarp;
+    uint8_t *out_buf = base_ptr + out_off + (part * 4 + quarter) * kF8OutWarp;
+    const uint32_t out_addr = base + out_off + (part * 4 + quarter) * kF8OutWarp;
     const size_t esize = g.c_dtype == kDtypeF32 ? 4 : 2;
     const bool vec_ok = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && (g.c_stride * esize) % 16 == 0;
     const int n_blocks = (g.N + 127) / 128;
     const uint32_t leader_acc_empty0 = map_to_cta(acc_empty_bar(0), 0);
-    RingPos buf;
+    RingPos pos, buf;
     bool ok = true;
     for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
       const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
-      const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128, n0 = tc.n_blk * kF8BN + half * 128;
+      const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128, n0 = tc.n_blk * kF8BN + part * kF8Cols;
       const int m = m0 + row;
       // rows and columns past the end compute zeros (TMA fills their codes with them) and are not stored: any scale will do
       const float *sa_p = g.sa + min(m, g.M - 1);
       const float *sw_p = g.sw + static_cast<size_t>(min(n0 / 128, n_blocks - 1)) * g.sw_stride;
-      float bias[4];
+      float bias[kF8Cols / 32];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kF8Cols / 32; ++j) {
         const int n = n0 + j * 32 + lane;
         bias[j] = g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
       }
-      float2 acc[64];
+      float2 acc[kF8Cols / 2];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+      for (int j = 0; j < kF8Cols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
       // scales two groups ahead of their use
       float a0 = __ldg(sa_p), w0 = __ldg(sw_p), a1 = 0.0f, w1 = 0.0f;
       if (groups > 1) {
@@ -196,29 +193,27 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
           a1 = __ldg(sa_p + static_cast<size_t>(kb + 2) * g.sa_stride);
           w1 = __ldg(sw_p + kb + 2);
         }
-        ok = mbar_wait(acc_full_bar(buf.s), buf.ph, cta_abort, g.status, kStatusEpilogueTimeout);
+        ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
         if (!__all_sync(0xFFFFFFFFu, ok)) {  // a warp gives up as a whole
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * kF8BN + half * 128;
+        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * kF8BN + part * kF8Cols;
         const float2 s2 = make_float2(s, s);
-        // two register sets: the next sixteen columns are on their way while these are added
-        uint32_t p[2][16];
-        tmem_ld_32x32b_x16(t_acc, p[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < kF8Cols; c += 32) {
+          uint32_t p[32];
+          tmem_ld_32x32b_x32(t_acc + c, p);
           tmem_ld_wait();
-          if (c < 7) {
-            tmem_ld_32x32b_x16(t_acc + (c + 1) * 16, p[(c + 1) & 1]);
-          } else {  // the warp's last values of the group are in registers: the leader may overwrite them
+          if (c + 32 == kF8Cols) {  // the warp's last values of the group are in registers: the leader may overwrite them
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8u * buf.s);
           }
-          scale_add16(p[c & 1], s2, acc + c * 8);
+          scale_add32(p, s2, acc + c / 2);
         }
+        pos.advance(stages);
         buf.advance(2);
       }
       if (!ok) break;
@@ -227,7 +222,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
         __syncwarp();
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kF8Cols / 32; ++c) {
         float v[32];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -256,11 +251,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
         __syncwarp();
         if (lane == 0) {
           const int y = m0 + quarter * 32;
-          if (y < g.M) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (n0 + i * 64 < g.N) tma_store_2d(&g.map_c, out_addr + i * kOutPanel, n0 + i * 64, y);
-          }
+          if (y < g.M && n0 < g.N) tma_store_2d(&g.map_c, out_addr, n0, y);
           tma_store_commit();
         }
       }
