@@ -939,7 +939,7 @@ int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, 
   g.map_w = *m;
   cudaEvent_t ps = nullptr;
   if (ctx->before_launch(&ps)) return -1;
-  return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_small(g, ctx->stream));
+  return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_small(g, ctx->prop.multiProcessorCount, ctx->stream));
 }
 
 int h3b_selftest_expire_wait(h3b_ctx *ctx) {

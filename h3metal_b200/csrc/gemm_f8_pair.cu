@@ -11,10 +11,11 @@
 // accumulators of 256 columns let the MMAs of a group run while the group before is read.
 //
 // Roles per CTA (rank 0 = leader): warp 0 TMA producer (own 128 rows of A, own half of the 256 rows of W per group, bytes
-// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..19
-// epilogue: four lane quarters x four parts of 64 columns; the first four warps hand them most of their registers. 16-bit results are staged in shared memory as 128-byte-swizzled panels and stored by TMA
-// while the next tile runs; fp32 results and unaligned outputs are stored from registers. Set-up overlaps the kernel before
-// (programmatic stream serialization). All waits are bounded. No load uses multicast.
+// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..11
+// epilogue: four lane quarters x two halves of 128 columns; the first four warps hand them most of their registers. 16-bit
+// results are staged in shared memory as 128-byte-swizzled panels and stored by TMA while the next tile runs; fp32 results
+// and unaligned outputs are turned there and stored row by row. Set-up overlaps the kernel before (programmatic stream
+// serialization). All waits are bounded. No load uses multicast.
 #include <cuda.h>
 
 #include "gemm_common.cuh"
@@ -26,31 +27,64 @@ using namespace gemm;
 
 constexpr int kF8BN = 256;
 constexpr int kF8Stage = kABytes + 128 * kBKBytes;  // 32 KB: this CTA's rows of A and its half of W
-constexpr int kF8EpiWarps = 16;
-constexpr int kF8Cols = kF8BN / (kF8EpiWarps / 4);  // columns per epilogue thread
-static_assert(kF8Cols == 64, "a warp's columns are one staging panel and lie in one weight block");
+constexpr int kF8Stages = 5;
+constexpr int kF8EpiWarps = 8;
+constexpr int kF8Cols = kF8BN / (kF8EpiWarps / 4);  // columns per epilogue thread: 128, those of one weight block
 constexpr int kF8Threads = 128 + 32 * kF8EpiWarps;
-// Registers per thread after the split: 128 x 32 + 512 x 112 = 61440 = 640 x 96, what the launch was given.
-constexpr int kF8RegsIssue = 32, kF8RegsEpi = 112;
-constexpr int kF8OutWarp = kOutPanel;               // a warp's 32 rows x 64 two-byte columns
+// Registers per thread after the split: 128 x 104 + 256 x 200 = 64512 = 384 x 168, what the launch was
+// given. Neither side spills with these; 56 and 224 make the issuing warps spill and cost 6 % of the whole product.
+constexpr int kF8RegsIssue = 104, kF8RegsEpi = 200;
+constexpr int kF8OutWarp = 2 * kOutPanel;           // a warp's 32 rows x 128 two-byte columns
 constexpr int kF8OutBytes = kF8EpiWarps * kF8OutWarp;
 
-// acc += p * s for 32 columns, two at a time
-__device__ __forceinline__ void scale_add32(const uint32_t (&p)[32], float2 s2, float2 *acc) {
+// acc += p * s for 16 columns, two at a time
+__device__ __forceinline__ void scale_add16(const uint32_t (&p)[16], float2 s2, float2 *acc) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < 8; ++j)
     acc[j] = __ffma2_rn(make_float2(__uint_as_float(p[2 * j]), __uint_as_float(p[2 * j + 1])), s2, acc[j]);
 }
+// 32 columns of a warp's 32 rows, from (m, n) on, without TMA: turned in 4 KB of shared memory (piece p of row r sits at
+// p ^ (r & 7)) so that a store instruction writes whole rows. A thread's own row, stored as it lies in registers, would
+// touch 32 lines per instruction: 575 against 204 us at 4608 x 11520 x 3840.
+__device__ __forceinline__ void store_chunk(const GemmF8Launch &g, float *buf, int lane, const float (&v)[32], int m, int n) {
+  __syncwarp();  // the chunk before has been read
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    reinterpret_cast<float4 *>(buf)[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  __syncwarp();
+  if (g.c_dtype == kDtypeF32 && n + 32 <= g.N && reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.c_stride % 4 == 0) {
+    const int q = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // four rows per instruction
+      const int r = 4 * i + (lane >> 3);
+      const float4 x = reinterpret_cast<const float4 *>(buf)[r * 8 + (q ^ (r & 7))];
+      if (m + r < g.M) *reinterpret_cast<float4 *>(static_cast<float *>(g.c) + static_cast<size_t>(m + r) * g.c_stride + n + 4 * q) = x;
+    }
+  } else if (n + lane < g.N) {
+    const int rows = min(32, g.M - m);
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      const float x = buf[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4 + (lane & 3)];
+      const size_t at = static_cast<size_t>(m + r) * g.c_stride + n + lane;
+      if (g.c_dtype == kDtypeF32) static_cast<float *>(g.c)[at] = x;
+      else if (g.c_dtype == kDtypeBf16) static_cast<__nv_bfloat16 *>(g.c)[at] = __float2bfloat16_rn(x);
+      else static_cast<__half *>(g.c)[at] = __float2half_rn(x);
+    }
+  }
+}
 
+// STAGED: 16-bit results by TMA (g.map_c). A kernel of its own, because the other way out costs the main loop registers.
+template <bool STAGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
-gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
+gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t *base_ptr = smem_raw + (base - raw_addr);
-  // [ring: stages x 32 KB][staged stores: 64 KB, optional][barriers 256 B]
-  const uint32_t out_off = stages * kF8Stage;
-  const uint32_t bars_off = out_off + (g.tma_store ? kF8OutBytes : 0);
+  // [ring: 5 x 32 KB][staging of results: 64 KB][barriers 256 B]
+  constexpr int stages = kF8Stages;
+  constexpr uint32_t out_off = stages * kF8Stage;
+  constexpr uint32_t bars_off = out_off + kF8OutBytes;
   const uint32_t bars = base + bars_off;
   auto full_bar = [&](int i) { return bars + 8u * i; };
   auto done_bar = [&](int i) { return bars + 64u + 8u * i; };
@@ -69,7 +103,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
   if (warp == 0 && lane == 0) {
     tma_prefetch_descriptor(&g.map_a);
     tma_prefetch_descriptor(&g.map_w);
-    if (g.tma_store) tma_prefetch_descriptor(&g.map_c);
+    if (STAGED) tma_prefetch_descriptor(&g.map_c);
     for (int i = 0; i < stages; ++i) {
       mbar_init(full_bar(i), 1);  // the leader's producer arms it; bytes arrive from both CTAs
       mbar_init(done_bar(i), 1);  // one commit arrival per use
@@ -133,10 +167,10 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
         bool ok = true;
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
           for (int kb = 0; kb < groups; ++kb) {
-            ok = mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout);
-            if (!ok) break;
             const uint32_t s = pos.s;
             ok = mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout);
+            if (!ok) break;
+            ok = mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout);  // the later of the two
             if (!ok) break;
             tc_fence_after_sync();
             const uint64_t ad = ad0 + static_cast<uint64_t>(s * (kF8Stage >> 4));
@@ -155,69 +189,62 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8RegsEpi));
     const int quarter = warp & 3, part = (warp - 4) >> 2;
     const int row = quarter * 32 + lane;
-    const bool staged = g.tma_store != 0;
-    uint8_t *out_buf = base_ptr + out_off + (part * 4 + quarter) * kF8OutWarp;
-    const uint32_t out_addr = base + out_off + (part * 4 + quarter) * kF8OutWarp;
-    const size_t esize = g.c_dtype == kDtypeF32 ? 4 : 2;
-    const bool vec_ok = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && (g.c_stride * esize) % 16 == 0;
     const int n_blocks = (g.N + 127) / 128;
     const uint32_t leader_acc_empty0 = map_to_cta(acc_empty_bar(0), 0);
-    RingPos pos, buf;
+    RingPos pos;
+    uint32_t buf = 0;
     bool ok = true;
     for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
       const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
       const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128, n0 = tc.n_blk * kF8BN + part * kF8Cols;
       const int m = m0 + row;
       // rows and columns past the end compute zeros (TMA fills their codes with them) and are not stored: any scale will do
-      const float *sa_p = g.sa + min(m, g.M - 1);
-      const float *sw_p = g.sw + static_cast<size_t>(min(n0 / 128, n_blocks - 1)) * g.sw_stride;
+      const int m_s = min(m, g.M - 1), n_s = min(n0 / 128, n_blocks - 1);
+      float2 acc[kF8Cols / 2];
+#pragma unroll
+      for (int j = 0; j < kF8Cols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+      // the next group's scales are fetched while this group's are waited for and used
+      float a_s = __ldg(g.sa + m_s), w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride);
+#pragma unroll 1
+      for (int kb = 0; kb < groups; ++kb) {
+        const float s = __fmul_rn(a_s, w_s);
+        if (kb + 1 < groups) {
+          a_s = __ldg(g.sa + static_cast<size_t>(kb + 1) * g.sa_stride + m_s);
+          w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + kb + 1);
+        }
+        ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
+        ok = __all_sync(0xFFFFFFFFu, ok);  // a warp gives up as a whole
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kF8BN + part * kF8Cols;
+        const float2 s2 = make_float2(s, s);
+        // two register sets: the next 16 columns are on their way while these are added
+        uint32_t p[2][16];
+        tmem_ld_32x32b_x16(t_acc, p[0]);
+#pragma unroll
+        for (int c = 0; c < kF8Cols / 16; ++c) {
+          tmem_ld_wait();
+          if (c + 1 < kF8Cols / 16) tmem_ld_32x32b_x16(t_acc + (c + 1) * 16, p[(c + 1) & 1]);
+          else {  // the warp's last values of the group are in registers: the leader may overwrite them
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8u * buf);
+          }
+          scale_add16(p[c & 1], s2, acc + c * 8);
+        }
+        pos.advance(stages);
+        buf ^= 1u;
+      }
+      if (!ok) break;
       float bias[kF8Cols / 32];
 #pragma unroll
       for (int j = 0; j < kF8Cols / 32; ++j) {
         const int n = n0 + j * 32 + lane;
         bias[j] = g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
       }
-      float2 acc[kF8Cols / 2];
-#pragma unroll
-      for (int j = 0; j < kF8Cols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
-      // scales two groups ahead of their use
-      float a0 = __ldg(sa_p), w0 = __ldg(sw_p), a1 = 0.0f, w1 = 0.0f;
-      if (groups > 1) {
-        a1 = __ldg(sa_p + g.sa_stride);
-        w1 = __ldg(sw_p + 1);
-      }
-      for (int kb = 0; kb < groups; ++kb) {
-        const float s = __fmul_rn(a0, w0);
-        a0 = a1; w0 = w1;
-        if (kb + 2 < groups) {
-          a1 = __ldg(sa_p + static_cast<size_t>(kb + 2) * g.sa_stride);
-          w1 = __ldg(sw_p + kb + 2);
-        }
-        ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {  // a warp gives up as a whole
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * kF8BN + part * kF8Cols;
-        const float2 s2 = make_float2(s, s);
-#pragma unroll
-        for (int c = 0; c < kF8Cols; c += 32) {
-          uint32_t p[32];
-          tmem_ld_32x32b_x32(t_acc + c, p);
-          tmem_ld_wait();
-          if (c + 32 == kF8Cols) {  // the warp's last values of the group are in registers: the leader may overwrite them
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8u * buf.s);
-          }
-          scale_add32(p, s2, acc + c / 2);
-        }
-        pos.advance(stages);
-        buf.advance(2);
-      }
-      if (!ok) break;
-      if (staged) {  // the panels of the tile before must have been read out of shared memory
+      uint8_t *out_buf = base_ptr + out_off + (part * 4 + quarter) * kF8OutWarp;
+      const uint32_t out_addr = base + out_off + (part * 4 + quarter) * kF8OutWarp;
+      if constexpr (STAGED) {  // the panels of the tile before must have been read out of shared memory
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
       }
@@ -233,30 +260,28 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], __shfl_sync(0xFFFFFFFFu, bias[c], j));
         }
-        if (staged) {
+        if constexpr (STAGED) {
           if (g.c_dtype == kDtypeBf16) stage_out32<__nv_bfloat16>(out_buf, c, lane, v);
           else stage_out32<__half>(out_buf, c, lane, v);
         } else {
-          const int n = n0 + c * 32, n_valid = g.N - n;
-          if (m < g.M && n_valid > 0) {
-            const size_t at = static_cast<size_t>(m) * g.c_stride + n;
-            if (g.c_dtype == kDtypeF32) store_segment(static_cast<float *>(g.c) + at, v, n_valid, vec_ok);
-            else if (g.c_dtype == kDtypeBf16) store_segment(static_cast<__nv_bfloat16 *>(g.c) + at, v, n_valid, vec_ok);
-            else store_segment(static_cast<__half *>(g.c) + at, v, n_valid, vec_ok);
-          }
+          store_chunk(g, reinterpret_cast<float *>(out_buf), lane, v, m0 + quarter * 32, n0 + c * 32);
         }
       }
-      if (staged) {
+      if constexpr (STAGED) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           const int y = m0 + quarter * 32;
-          if (y < g.M && n0 < g.N) tma_store_2d(&g.map_c, out_addr, n0, y);
+          if (y < g.M) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (n0 + i * 64 < g.N) tma_store_2d(&g.map_c, out_addr + i * kOutPanel, n0 + i * 64, y);
+          }
           tma_store_commit();
         }
       }
     }
-    if (staged && lane == 0) tma_store_wait_all();
+    if (STAGED && lane == 0) tma_store_wait_all();
     __syncwarp();
   }
 
@@ -269,43 +294,41 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
   }
 }
 
-size_t pair_bytes(int stages, bool staged) {
-  return 1024 + static_cast<size_t>(stages) * kF8Stage + (staged ? kF8OutBytes : 0) + kBarrierBytes;
-}
-int pair_stages(bool staged) { return staged ? 5 : 6; }
+constexpr size_t kF8Smem = 1024 + static_cast<size_t>(kF8Stages) * kF8Stage + kF8OutBytes + kBarrierBytes;
+static_assert(kF8Smem <= 232448, "ring and staging share 227 KB");
 
 }  // namespace
 
 cudaError_t gemm_f8_pair_configure(int *clusters) {
-  static_assert(1024 + 5 * kF8Stage + kF8OutBytes + kBarrierBytes <= 232448, "ring and staging share 227 KB");
   *clusters = 0;
-  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(gemm_f8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
   cfg.blockDim = dim3(kF8Threads, 1, 1);
-  cfg.dynamicSmemBytes = pair_bytes(pair_stages(true), true);
+  cfg.dynamicSmemBytes = kF8Smem;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaOccupancyMaxActiveClusters(clusters, gemm_f8_pair_kernel, &cfg);
+  return cudaOccupancyMaxActiveClusters(clusters, gemm_f8_pair_kernel<true>, &cfg);
 }
 
 cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
-  const bool staged = g.tma_store != 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);  // the cluster shape (2, 1, 1) is part of the kernel's declaration
   cfg.blockDim = dim3(kF8Threads);
-  cfg.dynamicSmemBytes = pair_bytes(pair_stages(staged), staged);
+  cfg.dynamicSmemBytes = kF8Smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g.overlap ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel, g, pair_stages(staged));
+  return g.tma_store ? cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<true>, g) : cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<false>, g);
 }
 
 }  // namespace h3b

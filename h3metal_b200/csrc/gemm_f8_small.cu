@@ -24,14 +24,18 @@ using namespace gemm;
 
 constexpr int kWRows = 128;                     // weight rows per tile = MMA M = one scale block of W
 constexpr int kWBytes = kWRows * kBKBytes;      // 16 KB
-constexpr int kScaleSlots = 4;                  // groups whose activation scales are on their way
-constexpr int kSmallBars = 256;
+constexpr int kSmallBars = 512;
+constexpr int kSmallMaxStages = 12;
 
 template <int NT> struct Small {
   static constexpr int kStage = kWBytes + NT * kBKBytes;
-  static constexpr int kBufs = NT <= 64 ? 4 : 2;             // accumulators in tensor memory
-  static constexpr int kCols = NT * kBufs;                   // 64, 128, 256, 256
-  static constexpr int kScaleBytes = 4 * kScaleSlots * NT * 4;  // per epilogue warp
+  static constexpr int kEpiWarps = NT <= 32 ? 4 : NT / 8;    // four lane quarters x parts of up to 32 rows of A
+  static constexpr int kRows = NT / (kEpiWarps / 4);         // rows of A (accumulator columns) per epilogue thread
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kBufs = 4;                            // accumulators in tensor memory, at most
+  static constexpr int kCols = NT * kBufs;                   // 64 .. 512
+  static constexpr int kScaleBytes = kEpiWarps * 2 * kRows * 4;  // two slots per epilogue warp
+  static constexpr int kPerSm = NT <= 32 ? 3 : NT <= 64 ? 2 : 1; // CTAs an SM can hold (registers, tensor memory)
 };
 
 // fp32 value of the other CTA's shared memory
@@ -49,9 +53,10 @@ __device__ __forceinline__ void store_one(const GemmF8Launch &g, int m, int n, f
 }
 
 template <int NT>
-__global__ void __launch_bounds__(192, NT <= 16 ? 3 : NT <= 64 ? 2 : 1)
-gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
+__global__ void __launch_bounds__(Small<NT>::kThreads, Small<NT>::kPerSm)
+gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, const int bufs) {
   using S = Small<NT>;
+  constexpr int kRows = S::kRows;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -59,12 +64,10 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
   const uint32_t bars_off = stages * S::kStage;
   const uint32_t bars = base + bars_off;
   auto full_bar = [&](int i) { return bars + 8u * i; };
-  auto empty_bar = [&](int i) { return bars + 64u + 8u * i; };
-  auto acc_full_bar = [&](int i) { return bars + 128u + 8u * i; };
-  auto acc_empty_bar = [&](int i) { return bars + 160u + 8u * i; };
-  volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(base_ptr + bars_off + 192);
-  volatile int *cta_abort = reinterpret_cast<volatile int *>(base_ptr + bars_off + 196);
-  const uint32_t scales_off = bars_off + kSmallBars;
+  auto done_bar = [&](int i) { return bars + 128u + 8u * i; };
+  auto acc_empty_bar = [&](int i) { return bars + 256u + 8u * i; };
+  volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(base_ptr + bars_off + 288);
+  volatile int *cta_abort = reinterpret_cast<volatile int *>(base_ptr + bars_off + 292);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = g.split;
@@ -81,12 +84,9 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
     tma_prefetch_descriptor(&g.map_w);
     for (int i = 0; i < stages; ++i) {
       mbar_init(full_bar(i), 1);
-      mbar_init(empty_bar(i), 1);
+      mbar_init(done_bar(i), 1);  // one commit per use: the stage may be refilled, the accumulator read
     }
-    for (int i = 0; i < S::kBufs; ++i) {
-      mbar_init(acc_full_bar(i), 1);
-      mbar_init(acc_empty_bar(i), 4);
-    }
+    for (int i = 0; i < bufs; ++i) mbar_init(acc_empty_bar(i), S::kEpiWarps);
     *cta_abort = 0;
     fence_barrier_init();
   }
@@ -101,14 +101,16 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
   grid_dep_launch();
   grid_dep_wait();  // global memory is read and written from here on only
 
-  float acc[NT];  // epilogue threads: running sums of output channel n0 + row for NT rows of A
+  const int quarter = warp & 3, part = (warp - 2) >> 2;  // epilogue warps: TMEM lanes and rows of A
+  const int row = quarter * 32 + lane, n = n0 + row;     // their output channel
+  float acc[kRows];                                      // its running sums for rows m0 + part * kRows ..
   if (warp == 0) {
     if (lane == 0) {
       RingPos pos;
       uint32_t filled = 0;
       for (int kb = g_begin; kb < g_end; ++kb) {
         const uint32_t s = pos.s;
-        if (!mbar_wait(empty_bar(s), pos.ph ^ 1u, cta_abort, g.status, kStatusProducerTimeout)) break;
+        if (!mbar_wait(done_bar(s), pos.ph ^ 1u, cta_abort, g.status, kStatusProducerTimeout)) break;
         mbar_arrive_expect_tx(full_bar(s), S::kStage);
         const uint32_t dst = base + s * S::kStage;
         tma_load_2d(dst, &g.map_w, full_bar(s), kb * kBKBytes, n0);
@@ -131,102 +133,104 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
       const uint64_t ad0 = umma_smem_desc(base + kWBytes, 1024, 2);
       RingPos pos, buf;
       for (int kb = g_begin; kb < g_end; ++kb) {
-        if (!mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout)) break;
         const uint32_t s = pos.s;
         if (!mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout)) break;
+        if (!mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout)) break;
         tc_fence_after_sync();
         const uint64_t wd = wd0 + static_cast<uint64_t>(s * (S::kStage >> 4));
         const uint64_t ad = ad0 + static_cast<uint64_t>(s * (S::kStage >> 4));
         const uint32_t d = tmem_base + buf.s * NT;
 #pragma unroll
         for (int k = 0; k < kBKBytes / 32; ++k) umma_f8(d, wd + 2u * k, ad + 2u * k, idesc, k ? 1u : 0u);
-        umma_commit(empty_bar(s));
-        umma_commit(acc_full_bar(buf.s));
+        umma_commit(done_bar(s));
         pos.advance(stages);
-        buf.advance(S::kBufs);
+        buf.advance(bufs);
       }
     }
   } else {
-    const int quarter = warp & 3;
-    float *my_scales = reinterpret_cast<float *>(base_ptr + scales_off) + (warp - 2) * kScaleSlots * NT;
-    const uint32_t my_scales_addr = base + scales_off + (warp - 2) * kScaleSlots * NT * 4;
-    const float *sw_row = g.sw + static_cast<size_t>(n_blk) * g.sw_stride;
+    float *slots = reinterpret_cast<float *>(base_ptr + bars_off + kSmallBars) + (warp - 2) * 2 * kRows;
+    const float *sw_p = g.sw + static_cast<size_t>(n_blk) * g.sw_stride;
+    // Lane t of the warp fetches the scale of its t-th row of A four groups ahead; the product with the weight block's scale
+    // goes through a slot of shared memory to all lanes. Rows past the end read another row's scale: their sums are zeros
+    // (TMA fills their codes with them) and are not stored.
+    const int t = part * kRows + lane;
+    const float *sa_p = g.sa + (lane < kRows && m0 + t < g.M ? m0 + t : m0);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
-    // the activation scales of group kb on their way to this warp's slot; rows past the end read as 0
-    auto fetch = [&](int kb) {
-      if (kb < g_end) {
+    for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
+    // Unrolled over the fetches in flight, so that a scale stays in the register that its load wrote: moving it on would
+    // wait for the load.
+    constexpr int kAhead = 4;
+    float a_s[kAhead], w_s[kAhead];
 #pragma unroll
-        for (int t = lane; t < NT; t += 32) {
-          const bool ok = m0 + t < g.M;
-          cp_async_4(my_scales_addr + ((kb & (kScaleSlots - 1)) * NT + t) * 4,
-                     g.sa + static_cast<size_t>(kb) * g.sa_stride + (ok ? m0 + t : 0), ok);
-        }
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kScaleSlots - 1; ++i) fetch(g_begin + i);
-    float ws = __ldg(sw_row + g_begin);
-    RingPos buf;
-    for (int kb = g_begin; kb < g_end; ++kb) {
-      __syncwarp();  // every lane is done with the slot that is filled next
-      fetch(kb + kScaleSlots - 1);
-      const float ws_next = kb + 1 < g_end ? __ldg(sw_row + kb + 1) : 0.0f;
-      cp_async_wait<kScaleSlots - 1>();
-      __syncwarp();
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(acc_full_bar(buf.s), buf.ph, cta_abort, g.status, kStatusEpilogueTimeout))) break;
-      tc_fence_after_sync();
-      const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * NT;
-      const float *s4 = my_scales + (kb & (kScaleSlots - 1)) * NT;
-      constexpr int kChunk = NT < 32 ? 16 : 32;
-#pragma unroll
-      for (int c = 0; c < NT; c += kChunk) {
-        uint32_t p[kChunk];
-        if constexpr (kChunk == 16) tmem_ld_32x32b_x16(t_acc + c, p);
-        else tmem_ld_32x32b_x32(t_acc + c, p);
-        tmem_ld_wait();
-        if (c + kChunk == NT) {  // the group's last values are in registers
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty_bar(buf.s));
-        }
-#pragma unroll
-        for (int j = 0; j < kChunk; j += 4) {
-          const float4 s = *reinterpret_cast<const float4 *>(s4 + c + j);
-          acc[c + j] = __fmaf_rn(__uint_as_float(p[j]), __fmul_rn(s.x, ws), acc[c + j]);
-          acc[c + j + 1] = __fmaf_rn(__uint_as_float(p[j + 1]), __fmul_rn(s.y, ws), acc[c + j + 1]);
-          acc[c + j + 2] = __fmaf_rn(__uint_as_float(p[j + 2]), __fmul_rn(s.z, ws), acc[c + j + 2]);
-          acc[c + j + 3] = __fmaf_rn(__uint_as_float(p[j + 3]), __fmul_rn(s.w, ws), acc[c + j + 3]);
-        }
-      }
-      ws = ws_next;
-      buf.advance(S::kBufs);
+    for (int u = 0; u < kAhead; ++u) {
+      const bool have = g_begin + u < g_end;
+      a_s[u] = have ? __ldg(sa_p + static_cast<size_t>(g_begin + u) * g.sa_stride) : 0.0f;
+      w_s[u] = have ? __ldg(sw_p + g_begin + u) : 0.0f;
     }
-    cp_async_wait<0>();
+    RingPos pos, buf;
+    bool ok = true;
+    for (int kb0 = g_begin; ok && kb0 < g_end; kb0 += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int kb = kb0 + u;
+        if (kb >= g_end) break;
+        float *slot = slots + (u & 1) * kRows;
+        if (lane < kRows) slot[lane] = __fmul_rn(a_s[u], w_s[u]);
+        if (kb + kAhead < g_end) {
+          a_s[u] = __ldg(sa_p + static_cast<size_t>(kb + kAhead) * g.sa_stride);
+          w_s[u] = __ldg(sw_p + kb + kAhead);
+        }
+        __syncwarp();  // this slot is written, and every lane is done with the other one
+        ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
+        ok = __all_sync(0xFFFFFFFFu, ok);  // a warp gives up as a whole
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf.s * NT + part * kRows;
+        uint32_t p[kRows];
+        if constexpr (kRows == 16) tmem_ld_32x32b_x16(t_acc, p);
+        else tmem_ld_32x32b_x32(t_acc, p);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty_bar(buf.s));
+#pragma unroll
+        for (int j = 0; j < kRows; j += 4) {
+          const float4 s = *reinterpret_cast<const float4 *>(slot + j);
+          acc[j] = __fmaf_rn(__uint_as_float(p[j]), s.x, acc[j]);
+          acc[j + 1] = __fmaf_rn(__uint_as_float(p[j + 1]), s.y, acc[j + 1]);
+          acc[j + 2] = __fmaf_rn(__uint_as_float(p[j + 2]), s.z, acc[j + 2]);
+          acc[j + 3] = __fmaf_rn(__uint_as_float(p[j + 3]), s.w, acc[j + 3]);
+        }
+        pos.advance(stages);
+        buf.advance(bufs);
+      }
+    }
   }
 
-  const int row = (warp & 3) * 32 + lane, n = n0 + row;  // epilogue threads: their output channel
   const float bias = warp >= 2 && g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
   if (split == 1) {
     if (warp >= 2 && n < g.N && !*cta_abort) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (m0 + t < g.M) store_one(g, m0 + t, n, __fadd_rn(acc[t], bias));
+      for (int j = 0; j < kRows; ++j) {
+        const int m = m0 + part * kRows + j;
+        if (m < g.M) store_one(g, m, n, __fadd_rn(acc[j], bias));
+      }
     }
   } else {
-    // every copy has landed and every MMA has read it (the last group's accumulator has been waited for, by all four
-    // epilogue warps before any of them can pass the barrier below), so the ring holds the partial sums: [row of A][128]
-    float *part = reinterpret_cast<float *>(base_ptr);
+    // every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
+    // any of them can pass the barrier below), so the ring holds the partial sums: [row of A][128]
+    float *sums = reinterpret_cast<float *>(base_ptr);
     __syncthreads();
     if (warp >= 2) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) part[t * kWRows + row] = acc[t];
+      for (int j = 0; j < kRows; ++j) sums[(part * kRows + j) * kWRows + row] = acc[j];
     }
+    __syncwarp();
     cluster_sync_all();
     if (warp >= 2 && n < g.N && !*cta_abort) {
-      const int t_begin = NT * rank / split, t_end = NT * (rank + 1) / split;
-      for (int t = t_begin; t < t_end && m0 + t < g.M; ++t) {
+      // this CTA finishes the rows t = rank, rank + split, ..: its epilogue warps take them in turn
+      const int rows_here = min(NT, g.M - m0);
+      for (int t = rank + split * part; t < rows_here; t += split * (S::kEpiWarps / 4)) {
         float sum = 0.0f;
         for (int q = 0; q < split; ++q)
           sum = __fadd_rn(sum, ld_cluster_f32(map_to_cta(base + (t * kWRows + row) * 4, q)));
@@ -245,12 +249,24 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages) {
 }
 
 template <int NT>
-cudaError_t launch_nt(const GemmF8Launch &g, int stages, cudaStream_t stream) {
+cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
+  using S = Small<NT>;
   cudaLaunchConfig_t cfg = {};
-  const int n_tiles = (g.N + kWRows - 1) / kWRows;
-  cfg.gridDim = dim3(static_cast<unsigned>(n_tiles) * g.m_tiles * g.split);
-  cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = 1024 + static_cast<size_t>(stages) * Small<NT>::kStage + kSmallBars + Small<NT>::kScaleBytes;
+  const unsigned grid = static_cast<unsigned>((g.N + kWRows - 1) / kWRows) * g.m_tiles * g.split;
+  // Ring depth: what is left of an SM's 228 KB for each of the CTAs that share it, and no more than there are groups.
+  const int want = static_cast<int>((grid + sms - 1) / sms);
+  const int per_sm = want < S::kPerSm ? want : S::kPerSm;
+  const int fixed = 1024 + kSmallBars + S::kScaleBytes;
+  const int room = 233472 / per_sm - 1024;  // the runtime keeps 1 KB per CTA
+  int stages = (room - fixed) / S::kStage;
+  const int groups = ((g.K + kBKBytes - 1) / kBKBytes + g.split - 1) / g.split;
+  if (stages > groups) stages = groups;
+  if (stages > kSmallMaxStages) stages = kSmallMaxStages;
+  const int for_sums = g.split > 1 ? (NT * kWRows * 4 + S::kStage - 1) / S::kStage : 1;  // the ring also holds the partial sums
+  if (stages < for_sums) stages = for_sums;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = fixed + static_cast<size_t>(stages) * S::kStage;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -259,7 +275,10 @@ cudaError_t launch_nt(const GemmF8Launch &g, int stages, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g.overlap ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, gemm_f8_small_kernel<NT>, g, stages);
+  // A stage's barrier tells its uses apart by their parity alone. The epilogue, which waits on it too, must therefore be less
+  // than a whole ring behind the MMAs, and it can be as many groups behind as there are accumulators.
+  const int bufs = stages < S::kBufs ? stages : S::kBufs;
+  return cudaLaunchKernelEx(&cfg, gemm_f8_small_kernel<NT>, g, stages, bufs);
 }
 
 }  // namespace
@@ -274,13 +293,12 @@ cudaError_t gemm_f8_small_configure() {
   return cudaSuccess;
 }
 
-cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, cudaStream_t stream) {
-  // ring depth: three, two or one CTA per SM share its 227 KB
+cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   switch (g.nt) {
-    case 16: return launch_nt<16>(g, 4, stream);
-    case 32: return launch_nt<32>(g, 5, stream);
-    case 64: return launch_nt<64>(g, 4, stream);
-    default: return launch_nt<128>(g, 6, stream);
+    case 16: return launch_nt<16>(g, sms, stream);
+    case 32: return launch_nt<32>(g, sms, stream);
+    case 64: return launch_nt<64>(g, sms, stream);
+    default: return launch_nt<128>(g, sms, stream);
   }
 }
 

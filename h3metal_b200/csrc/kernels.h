@@ -201,7 +201,7 @@ struct GemmF8Launch {
   int *status;
 };
 cudaError_t gemm_f8_small_configure();
-cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, cudaStream_t stream);
+cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, int sms, cudaStream_t stream);
 // CTA pairs on 256 x 256 tiles; *clusters: pairs that can be resident at once
 cudaError_t gemm_f8_pair_configure(int *clusters);
 cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream);
