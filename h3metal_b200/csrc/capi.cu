@@ -904,7 +904,7 @@ int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, 
   g.c_dtype = c_dtype; g.M = M; g.N = N; g.K = K;
   g.overlap = (ctx->overlap != 0 && !ctx->profile) ? 1 : 0;
   g.status = ctx->status_dev;
-  const bool pair = M > 128 && N > 128 && ctx->f8_pair_clusters > 0;
+  const bool pair = h3b::gemm_f8_choose(g, ctx->prop.multiProcessorCount, ctx->f8_pair_clusters);
   const CUtensorMap *m;
   if (pair) {
     g.m_tiles = (M - 1) / 256 + 1;
@@ -929,9 +929,6 @@ int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, 
     const int clusters = static_cast<int>(tiles < ctx->f8_pair_clusters ? tiles : ctx->f8_pair_clusters);
     return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_pair(g, clusters, ctx->stream));
   }
-  g.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  g.m_tiles = (M - 1) / g.nt + 1;
-  g.split = 1;
   if (((N - 1LL) / 128 + 1) * g.m_tiles * g.split > 0x7FFFFFFFLL) return fail("gemm_f8: too many tiles for one launch");
   if (!(m = ctx->tensor_map(A, h3b::kDtypeI8, K, M, a_stride, 128, g.nt, 128))) return -1;
   g.map_a = *m;

@@ -168,9 +168,10 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
           for (int kb = 0; kb < groups; ++kb) {
             const uint32_t s = pos.s;
-            ok = mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout);
+            const bool full = mbar_test(full_bar(s), pos.ph), free = mbar_test(acc_empty_bar(buf.s), buf.ph ^ 1u);
+            ok = full || mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout);
             if (!ok) break;
-            ok = mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout);  // the later of the two
+            ok = free || mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout);
             if (!ok) break;
             tc_fence_after_sync();
             const uint64_t ad = ad0 + static_cast<uint64_t>(s * (kF8Stage >> 4));

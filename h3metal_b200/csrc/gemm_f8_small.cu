@@ -134,8 +134,10 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
       RingPos pos, buf;
       for (int kb = g_begin; kb < g_end; ++kb) {
         const uint32_t s = pos.s;
-        if (!mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout)) break;
-        if (!mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout)) break;
+        // two polls in flight at once: a barrier's answer takes about 80 cycles, a third of the instructions' own issue
+        const bool full = mbar_test(full_bar(s), pos.ph), free = mbar_test(acc_empty_bar(buf.s), buf.ph ^ 1u);
+        if (!full && !mbar_wait(full_bar(s), pos.ph, cta_abort, g.status, kStatusMmaTimeout)) break;
+        if (!free && !mbar_wait(acc_empty_bar(buf.s), buf.ph ^ 1u, cta_abort, g.status, kStatusMmaTimeout)) break;
         tc_fence_after_sync();
         const uint64_t wd = wd0 + static_cast<uint64_t>(s * (S::kStage >> 4));
         const uint64_t ad = ad0 + static_cast<uint64_t>(s * (S::kStage >> 4));
@@ -282,6 +284,33 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// Which kernel, and for few rows which tile height and how many CTAs share K. Times in nanoseconds, measured on B200 as
+// back-to-back launches (M x N x K: this kernel / CTA pairs, us): 256 x 3840 x 3840: 16.4 / 17.5; 512 x 3840 x 10240: 42.5 /
+// 38.6; 1024 x 3840 x 10240: 84.6 / 40.2; 512 x 20480 x 3840: 97.3 / 47.6. Both follow
+//   launch + (groups a CTA works through) * (time of a group),
+// a group taking 0.45 us on pairs and 0.475 us on 128-row tiles here.
+bool gemm_f8_choose(GemmF8Launch &g, int sms, int pair_clusters) {
+  const long long groups = (g.K + kBKBytes - 1) / kBKBytes;
+  const long long n_tiles = (static_cast<long long>(g.N) + kWRows - 1) / kWRows;
+  g.nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
+  g.m_tiles = (g.M - 1) / g.nt + 1;
+  const long long tiles = n_tiles * g.m_tiles;
+  // K is split while the parts still run side by side: 1 x 11520 x 3840 takes 13.0 / 11.6 / 10.3 / 13.7 us with 1 / 2 / 4 / 8
+  // parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 29.0 / 18.6 / 12.3 / 10.7 (30 tiles). Where the tiles
+  // alone fill the SMs a split only adds the exchange: 16 x 20480 x 3840 takes 16.1 / 17.7 (160 tiles).
+  const int per_sm = g.nt <= 32 ? 3 : g.nt <= 64 ? 2 : 1;
+  const long long slots = static_cast<long long>(sms) * per_sm;
+  g.split = 1;
+  if (tiles < sms)
+    while (g.split < 8 && tiles * g.split * 2 <= slots && g.split * 2 <= groups) g.split *= 2;
+  if (g.nt < 128 || pair_clusters <= 0) return false;
+  const long long waves = (tiles * g.split + slots - 1) / slots;
+  const long long here = 4500 + (g.split > 1 ? 1500 : 0) + waves * ((groups + g.split - 1) / g.split) * 475;
+  const long long pair_tiles = ((g.M - 1LL) / 256 + 1) * ((g.N - 1LL) / 256 + 1);
+  const long long pairs = 5000 + (pair_tiles + pair_clusters - 1) / pair_clusters * groups * 450;
+  return pairs < here;
+}
 
 cudaError_t gemm_f8_small_configure() {
   cudaError_t e;

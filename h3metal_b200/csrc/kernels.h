@@ -200,6 +200,8 @@ struct GemmF8Launch {
   int overlap;
   int *status;
 };
+// Fills in nt, m_tiles and split for few rows; true where CTA pairs are the faster choice.
+bool gemm_f8_choose(GemmF8Launch &g, int sms, int pair_clusters);
 cudaError_t gemm_f8_small_configure();
 cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, int sms, cudaStream_t stream);
 // CTA pairs on 256 x 256 tiles; *clusters: pairs that can be resident at once
