@@ -34,60 +34,79 @@ constexpr int kGroup = 128;   // channels per scale
 constexpr float kTop = 448.0f;
 constexpr float kTiny = 1.17549435e-38f;  // 2^-126
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// Sixteen consecutive values at p, of which the first n (>= 1) exist; the others read as 0. vec: p is 16-byte aligned.
+// Sixteen consecutive values of type T as they lie in memory: two per 32-bit word, or one.
 template <typename T>
-__device__ __forceinline__ void load_piece(const T *p, int n, bool vec, float (&v)[kPiece]) {
-  if (vec && n >= kPiece) {
-    constexpr int kPer = 16 / sizeof(T);
+struct Raw {
+  static constexpr int kWords = kPiece * sizeof(T) / 4;
+  uint32_t w[kWords];
+  // The first n values at p (n >= 1); the others read as 0. vec: p is 16-byte aligned.
+  __device__ __forceinline__ void load(const T *p, int n, bool vec) {
+    if (vec && n >= kPiece) {
 #pragma unroll
-    for (int q = 0; q < kPiece / kPer; ++q) {
-      const uint4 raw = reinterpret_cast<const uint4 *>(p)[q];
-      T e[kPer];
-      memcpy(e, &raw, 16);
+      for (int q = 0; q < kWords / 4; ++q) {
+        const uint4 u = reinterpret_cast<const uint4 *>(p)[q];
+        w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) v[q * kPer + i] = to_f32(e[i]);
+      for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        if (i >= n) continue;
+        if constexpr (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+        else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
   }
-}
+  __device__ __forceinline__ void store(T *p, int n) const {
+    if (n >= kPiece) {
+#pragma unroll
+      for (int q = 0; q < kWords / 4; ++q)
+        reinterpret_cast<uint4 *>(p)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        if (i >= n) continue;
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(p)[i] = w[i];
+        else reinterpret_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+  // Values 2 i and 2 i + 1, exactly. All arithmetic below works on such pairs (packed fp32 instructions: half the issue slots,
+  // each half rounded like the scalar operation): the kernels are otherwise bound by issue.
+  __device__ __forceinline__ float2 get(int i) const {
+    if constexpr (std::is_same<T, float>::value) {
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      __half2 h;
+      memcpy(&h, &w[i], 4);
+      return __half22float2(h);
+    } else {
+      return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+  }
+  __device__ __forceinline__ void set(int i, float2 v) {
+    if constexpr (std::is_same<T, float>::value) {
+      w[2 * i] = __float_as_uint(v.x);
+      w[2 * i + 1] = __float_as_uint(v.y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(v.x, v.y);
+      memcpy(&w[i], &h, 4);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+      memcpy(&w[i], &h, 4);
+    }
+  }
+};
 
-template <typename T>
-__device__ __forceinline__ void store_piece(T *p, int n, const float (&v)[kPiece]) {
-  if (n >= kPiece) {
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int q = 0; q < kPiece / kPer; ++q) {
-      T e[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) e[i] = from_f32<T>(v[q * kPer + i]);
-      uint4 raw;
-      memcpy(&raw, e, 16);
-      reinterpret_cast<uint4 *>(p)[q] = raw;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i)
-      if (i < n) p[i] = from_f32<T>(v[i]);
-  }
-}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // The scale of a group and the codes of this thread's piece. Called by the eight lanes of a group together; lanes past
 // the end of the row pass zeros and n <= 0.
-__device__ __forceinline__ void encode_piece(const float (&v)[kPiece], int n, uint8_t *dst, float *scale, bool first) {
+__device__ __forceinline__ void encode_piece(const float2 (&v)[kPiece / 2], int n, uint8_t *dst, float *scale, bool first) {
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPiece; ++i) top = fmaxf(top, fabsf(v[i]));
+  for (int i = 0; i < kPiece / 2; ++i) top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
 #pragma unroll
   for (int s = 1; s < 8; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
   const float sc = top > 0.0f ? fmaxf(__fdiv_rn(top, kTop), kTiny) : 1.0f;
@@ -96,10 +115,8 @@ __device__ __forceinline__ void encode_piece(const float (&v)[kPiece], int n, ui
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v[4 * j], rs), __fmul_rn(v[4 * j + 1], rs)),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(v[4 * j + 2], rs), __fmul_rn(v[4 * j + 3], rs)),
-                                                 __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * j], both(rs)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(__fmul2_rn(v[2 * j + 1], both(rs)), __NV_SATFINITE, __NV_E4M3);
     w[j] = lo | (hi << 16);
   }
   if (n >= kPiece) {
@@ -111,37 +128,54 @@ __device__ __forceinline__ void encode_piece(const float (&v)[kPiece], int n, ui
   }
 }
 
-// ---- quantiser: no statistics over the row, so a CTA simply takes the next 256 pieces -------------------------------
+// g / (1 + e^-g) for two gates, e^-g as 2^(-g log2 e). Relative error: the exponent's rounding, |g| * 2^-24 at most (|g| < 104;
+// beyond, e^-g is 0 or infinite), ex2 2^-22, rcp 2^-23, the other four roundings 2^-24 each. The denominator is
+// formed at a sixteenth, so that its reciprocal is never subnormal (ex2 and rcp flush those); the last product may be.
+__device__ __forceinline__ float2 silu(float2 g) {
+  const float2 h = __fmul2_rn(g, both(-1.44269504f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(h.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(h.y));
+  const float2 d = __ffma2_rn(e, both(0.0625f), both(0.0625f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return __fmul2_rn(g, __fmul2_rn(r, both(0.0625f)));
+}
+
+// ---- quantiser: no statistics over the row. A CTA covers blockDim.y rows (or part of one row, gridDim.y parts) --------
+struct QuantArgs {
+  const void *x;
+  uint8_t *out;
+  float *sa;
+  long long x_stride, out_stride, sa_stride;
+  int M, D;
+  bool gate_vec;  // the gates of a row start on a 16-byte boundary
+};
+
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(256) quant_f8_kernel(const T *x, long long x_stride, uint8_t *out, long long out_stride,
-                                                       float *sa, long long sa_stride, int M, int D, int per_row,
-                                                       bool gate_vec) {
+__global__ void __launch_bounds__(256) quant_f8_kernel(const QuantArgs p) {
   grid_dep_launch();
   grid_dep_wait();
-  // per_row: pieces of a row rounded up to whole groups, so that the lanes of a group stay together
-  const long long start = static_cast<long long>(blockIdx.x) * 256;
-  const long long m_first = start / per_row;
-  const int at = static_cast<int>(start - m_first * per_row) + threadIdx.x;
-  const long long m = m_first + at / per_row;
-  const int piece = at % per_row;
-  const bool have = m < M;
-  const int n = have ? D - piece * kPiece : 0;  // values of this piece that exist
-  float v[kPiece];
-#pragma unroll
-  for (int i = 0; i < kPiece; ++i) v[i] = 0.0f;
+  const int piece = blockIdx.y * blockDim.x + threadIdx.x;
+  const long long m = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int n = m < p.M ? p.D - piece * kPiece : 0;  // values of this piece that exist
+  float2 v[kPiece / 2];
   if (n > 0) {
-    const T *row = x + m * x_stride;
-    load_piece(row + piece * kPiece, n, true, v);
-    if (GATED) {
-      float g[kPiece];
-      load_piece(row + D + piece * kPiece, n, gate_vec, g);
+    const T *row = static_cast<const T *>(p.x) + m * p.x_stride + piece * kPiece;
+    Raw<T> x, g;
+    x.load(row, n, true);
+    if (GATED) g.load(row + p.D, n, p.gate_vec);
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i)
-        v[i] = __fmul_rn(v[i], __fdividef(g[i], __fadd_rn(1.0f, expf(-g[i]))));
+    for (int i = 0; i < kPiece / 2; ++i) {
+      v[i] = x.get(i);
+      if (GATED) v[i] = __fmul2_rn(v[i], silu(g.get(i)));
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPiece / 2; ++i) v[i] = both(0.0f);
   }
   const int group = piece >> 3;
-  encode_piece(v, n, out + m * out_stride + piece * kPiece, sa + group * sa_stride + m, have && (piece & 7) == 0);
+  encode_piece(v, n, p.out + m * p.out_stride + piece * kPiece, p.sa + group * p.sa_stride + m, n > 0 && (piece & 7) == 0);
 }
 
 // ---- norm: one CTA per row, C pieces per thread --------------------------------------------------------------------
@@ -157,10 +191,12 @@ struct RmsArgs {
 
 struct None {};
 
-__device__ __forceinline__ void load_gain(const RmsArgs &p, int at, int n, float (&w)[kPiece]) {
-  if (p.w_dtype == kDtypeF32) load_piece(static_cast<const float *>(p.w) + at, n, true, w);
-  else if (p.w_dtype == kDtypeBf16) load_piece(static_cast<const __nv_bfloat16 *>(p.w) + at, n, true, w);
-  else load_piece(static_cast<const __half *>(p.w) + at, n, true, w);
+template <typename T>
+__device__ __forceinline__ void scale_by(float2 (&v)[kPiece / 2], const void *w, int at, int n, float inv) {
+  Raw<T> g;
+  g.load(static_cast<const T *>(w) + at, n, true);
+#pragma unroll
+  for (int i = 0; i < kPiece / 2; ++i) v[i] = __fmul2_rn(__fmul2_rn(v[i], both(inv)), g.get(i));
 }
 
 template <typename TX, typename TY, int C>
@@ -171,26 +207,31 @@ __global__ void __launch_bounds__(512) rms_f8_kernel(const RmsArgs p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const long long m = blockIdx.x;
   constexpr bool kAdd = !std::is_same<TY, None>::value;
-  float v[C][kPiece];
-  float ss = 0.0f;
+  float2 v[C][kPiece / 2];
+  float2 ss2 = both(0.0f);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int at = (tid + c * blockDim.x) * kPiece, n = p.D - at;
-#pragma unroll
-    for (int i = 0; i < kPiece; ++i) v[c][i] = 0.0f;
     if (n > 0) {
-      load_piece(static_cast<const TX *>(p.x) + m * p.x_stride + at, n, true, v[c]);
+      Raw<TX> x;
+      x.load(static_cast<const TX *>(p.x) + m * p.x_stride + at, n, true);
       if constexpr (kAdd) {
-        float y[kPiece];
-        load_piece(static_cast<const TY *>(p.y) + m * p.y_stride + at, n, true, y);
+        Raw<TY> y;
+        y.load(static_cast<const TY *>(p.y) + m * p.y_stride + at, n, true);
 #pragma unroll
-        for (int i = 0; i < kPiece; ++i) v[c][i] = to_f32(from_f32<TX>(__fadd_rn(v[c][i], y[i])));
-        store_piece(static_cast<TX *>(p.res) + m * p.res_stride + at, n, v[c]);
+        for (int i = 0; i < kPiece / 2; ++i) x.set(i, __fadd2_rn(x.get(i), y.get(i)));
+        x.store(static_cast<TX *>(p.res) + m * p.res_stride + at, n);
       }
+#pragma unroll
+      for (int i = 0; i < kPiece / 2; ++i) v[c][i] = x.get(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiece / 2; ++i) v[c][i] = both(0.0f);
     }
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) ss = __fmaf_rn(v[c][i], v[c][i], ss);
+    for (int i = 0; i < kPiece / 2; ++i) ss2 = __ffma2_rn(v[c][i], v[c][i], ss2);
   }
+  float ss = __fadd_rn(ss2.x, ss2.y);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, s));
   if (warps > 1) {
@@ -204,10 +245,9 @@ __global__ void __launch_bounds__(512) rms_f8_kernel(const RmsArgs p) {
   for (int c = 0; c < C; ++c) {
     const int piece = tid + c * blockDim.x, at = piece * kPiece, n = p.D - at;
     if (n > 0) {
-      float w[kPiece];
-      load_gain(p, at, n, w);
-#pragma unroll
-      for (int i = 0; i < kPiece; ++i) v[c][i] = __fmul_rn(__fmul_rn(v[c][i], inv), w[i]);
+      if (p.w_dtype == kDtypeF32) scale_by<float>(v[c], p.w, at, n, inv);
+      else if (p.w_dtype == kDtypeBf16) scale_by<__nv_bfloat16>(v[c], p.w, at, n, inv);
+      else scale_by<__half>(v[c], p.w, at, n, inv);
     }
     const int group = piece >> 3;
     encode_piece(v[c], n, p.out + m * p.out_stride + at, p.sa + group * p.sa_stride + m,
@@ -216,10 +256,10 @@ __global__ void __launch_bounds__(512) rms_f8_kernel(const RmsArgs p) {
 }
 
 template <typename F, typename... Args>
-cudaError_t launch(F *kernel, unsigned grid, unsigned threads, bool overlap, cudaStream_t stream, Args... args) {
+cudaError_t launch(F *kernel, dim3 grid, dim3 threads, bool overlap, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -235,9 +275,9 @@ cudaError_t launch_rms(const RmsArgs &a, int M, bool overlap, cudaStream_t strea
   const int c = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
   const unsigned threads = ((pieces + c - 1) / c + 31) / 32 * 32;
   switch (c) {
-    case 1: return launch(rms_f8_kernel<TX, TY, 1>, M, threads, overlap, stream, a);
-    case 2: return launch(rms_f8_kernel<TX, TY, 2>, M, threads, overlap, stream, a);
-    default: return launch(rms_f8_kernel<TX, TY, 4>, M, threads, overlap, stream, a);
+    case 1: return launch(rms_f8_kernel<TX, TY, 1>, dim3(M), dim3(threads), overlap, stream, a);
+    case 2: return launch(rms_f8_kernel<TX, TY, 2>, dim3(M), dim3(threads), overlap, stream, a);
+    default: return launch(rms_f8_kernel<TX, TY, 4>, dim3(M), dim3(threads), overlap, stream, a);
   }
 }
 
@@ -251,17 +291,25 @@ cudaError_t launch_rms_y(const RmsArgs &a, int y_dtype, int M, bool overlap, cud
 
 template <typename T>
 cudaError_t launch_quant(const QuantF8Launch &q, bool overlap, cudaStream_t stream) {
-  const int per_row = (q.D + kGroup - 1) / kGroup * (kGroup / kPiece);
-  const long long blocks = (static_cast<long long>(q.M) * per_row + 255) / 256;
-  if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidConfiguration;
-  const bool gate_vec = (static_cast<long long>(q.D) * sizeof(T)) % 16 == 0;
-  const T *x = static_cast<const T *>(q.x);
-  uint8_t *out = static_cast<uint8_t *>(q.out);
-  if (q.gated)
-    return launch(quant_f8_kernel<T, true>, static_cast<unsigned>(blocks), 256, overlap, stream, x, q.x_stride, out,
-                  q.out_stride, q.sa, q.sa_stride, q.M, q.D, per_row, gate_vec);
-  return launch(quant_f8_kernel<T, false>, static_cast<unsigned>(blocks), 256, overlap, stream, x, q.x_stride, out,
-                q.out_stride, q.sa, q.sa_stride, q.M, q.D, per_row, gate_vec);
+  QuantArgs a;
+  a.x = q.x; a.out = static_cast<uint8_t *>(q.out); a.sa = q.sa;
+  a.x_stride = q.x_stride; a.out_stride = q.out_stride; a.sa_stride = q.sa_stride; a.M = q.M; a.D = q.D;
+  a.gate_vec = (static_cast<long long>(q.D) * sizeof(T)) % 16 == 0;
+  // About 256 threads: parts of a row of equal length, or several short rows. Whole warps, whole groups of eight lanes.
+  const int pieces = (q.D + kGroup - 1) / kGroup * (kGroup / kPiece);
+  const int parts = (pieces + 255) / 256;
+  int tx = (pieces + parts - 1) / parts, ty = 1;
+  if (tx <= 64) {
+    tx = (tx + 7) / 8 * 8;
+    ty = 256 / tx / 4 * 4;
+  } else {
+    tx = (tx + 31) / 32 * 32;
+    ty = 256 / tx;
+  }
+  const dim3 grid((q.M - 1) / ty + 1, (pieces + tx - 1) / tx), threads(tx, ty);
+  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+  if (q.gated) return launch(quant_f8_kernel<T, true>, grid, threads, overlap, stream, a);
+  return launch(quant_f8_kernel<T, false>, grid, threads, overlap, stream, a);
 }
 
 }  // namespace
