@@ -879,7 +879,7 @@ int h3b_rms_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, const
   r.x_dtype = x_dtype; r.y_dtype = y_dtype; r.w_dtype = w_dtype; r.M = M; r.D = D; r.eps = eps;
   cudaEvent_t ps = nullptr;
   if (ctx->before_launch(&ps)) return -1;
-  return ctx->after_launch("rms_f8 launch", h3b::launch_rms_f8(r, ctx->overlap != 0 && !ctx->profile, ctx->stream));
+  return ctx->after_launch("rms_f8 launch", h3b::launch_rms_f8(r, ctx->prop.multiProcessorCount, ctx->overlap != 0 && !ctx->profile, ctx->stream));
 }
 
 int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, int64_t sa_stride, const void *W,

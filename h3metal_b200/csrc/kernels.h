@@ -184,7 +184,7 @@ struct RmsF8Launch {
   float eps;
 };
 constexpr int kRmsF8MaxD = 32768;
-cudaError_t launch_rms_f8(const RmsF8Launch &r, bool overlap, cudaStream_t stream);
+cudaError_t launch_rms_f8(const RmsF8Launch &r, int sms, bool overlap, cudaStream_t stream);
 
 struct GemmF8Launch {
   CUtensorMap map_a;   // e4m3 [M][K], box nt x 128 bytes (pairs: 128 x 128), 128-byte swizzle

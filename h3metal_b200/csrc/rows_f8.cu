@@ -20,6 +20,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -39,9 +40,18 @@ template <typename T>
 struct Raw {
   static constexpr int kWords = kPiece * sizeof(T) / 4;
   uint32_t w[kWords];
-  // The first n values at p (n >= 1); the others read as 0. vec: p is 16-byte aligned.
-  __device__ __forceinline__ void load(const T *p, int n, bool vec) {
-    if (vec && n >= kPiece) {
+  // The first n values at p (n >= 1); the others read as 0. align: 16-byte or 32-byte boundary of p, else any. A piece of 16-bit
+  // values is ONE 32-byte access: with two of 16 bytes, each touches every second half of the warp's cache lines.
+  __device__ __forceinline__ void load(const T *p, int n, int align) {
+    if (align >= 32 && n >= kPiece) {
+#pragma unroll
+      for (int q = 0; q < kWords / 8; ++q)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[8 * q]), "=r"(w[8 * q + 1]), "=r"(w[8 * q + 2]), "=r"(w[8 * q + 3]), "=r"(w[8 * q + 4]),
+                       "=r"(w[8 * q + 5]), "=r"(w[8 * q + 6]), "=r"(w[8 * q + 7])
+                     : "l"(reinterpret_cast<const uint32_t *>(p) + 8 * q)
+                     : "memory");
+    } else if (align >= 16 && n >= kPiece) {
 #pragma unroll
       for (int q = 0; q < kWords / 4; ++q) {
         const uint4 u = reinterpret_cast<const uint4 *>(p)[q];
@@ -58,8 +68,15 @@ struct Raw {
       }
     }
   }
-  __device__ __forceinline__ void store(T *p, int n) const {
-    if (n >= kPiece) {
+  __device__ __forceinline__ void store(T *p, int n, int align) const {
+    if (align >= 32 && n >= kPiece) {
+#pragma unroll
+      for (int q = 0; q < kWords / 8; ++q)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t *>(p) + 8 * q),
+                     "r"(w[8 * q]), "r"(w[8 * q + 1]), "r"(w[8 * q + 2]), "r"(w[8 * q + 3]), "r"(w[8 * q + 4]),
+                     "r"(w[8 * q + 5]), "r"(w[8 * q + 6]), "r"(w[8 * q + 7])
+                     : "memory");
+    } else if (n >= kPiece) {
 #pragma unroll
       for (int q = 0; q < kWords / 4; ++q)
         reinterpret_cast<uint4 *>(p)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
@@ -149,7 +166,7 @@ struct QuantArgs {
   float *sa;
   long long x_stride, out_stride, sa_stride;
   int M, D;
-  bool gate_vec;  // the gates of a row start on a 16-byte boundary
+  int x_align, gate_align;  // boundaries on which the rows and their gates start: 32 or 16 bytes, or (gates) any
 };
 
 template <typename T, bool GATED>
@@ -163,8 +180,8 @@ __global__ void __launch_bounds__(256) quant_f8_kernel(const QuantArgs p) {
   if (n > 0) {
     const T *row = static_cast<const T *>(p.x) + m * p.x_stride + piece * kPiece;
     Raw<T> x, g;
-    x.load(row, n, true);
-    if (GATED) g.load(row + p.D, n, p.gate_vec);
+    x.load(row, n, p.x_align);
+    if (GATED) g.load(row + p.D, n, p.gate_align);
 #pragma unroll
     for (int i = 0; i < kPiece / 2; ++i) {
       v[i] = x.get(i);
@@ -178,80 +195,113 @@ __global__ void __launch_bounds__(256) quant_f8_kernel(const QuantArgs p) {
   encode_piece(v, n, p.out + m * p.out_stride + piece * kPiece, p.sa + group * p.sa_stride + m, n > 0 && (piece & 7) == 0);
 }
 
-// ---- norm: one CTA per row, C pieces per thread --------------------------------------------------------------------
+// ---- norm: a CTA has a row at a time, C pieces per thread --------------------------------------------------------------------
 struct RmsArgs {
   const void *x, *y, *w;
   void *res;
   uint8_t *out;
   float *sa;
   long long x_stride, y_stride, res_stride, out_stride, sa_stride;
-  int D, w_dtype;
+  int M, D, w_dtype, x_align, y_align, res_align, w_align;
   float eps;
 };
 
 struct None {};
 
 template <typename T>
-__device__ __forceinline__ void scale_by(float2 (&v)[kPiece / 2], const void *w, int at, int n, float inv) {
-  Raw<T> g;
-  g.load(static_cast<const T *>(w) + at, n, true);
+__device__ __forceinline__ void read_gain(float2 (&g)[kPiece / 2], const void *w, int at, int n, int align) {
+  Raw<T> raw;
+  raw.load(static_cast<const T *>(w) + at, n, align);
 #pragma unroll
-  for (int i = 0; i < kPiece / 2; ++i) v[i] = __fmul2_rn(__fmul2_rn(v[i], both(inv)), g.get(i));
+  for (int i = 0; i < kPiece / 2; ++i) g[i] = raw.get(i);
 }
 
-template <typename TX, typename TY, int C>
-__global__ void __launch_bounds__(512) rms_f8_kernel(const RmsArgs p) {
-  __shared__ float part[16];
+// blockDim.x threads have a row, blockDim.y rows go side by side. Where a thread has one piece, the row that comes next is on
+// its way while the current one is normed (x and y in registers, as they lie in memory), and the gain stays in registers:
+// read for every row, fp32 gains kept the L1 pipeline 73 % busy. Registers decide how many rows an SM holds: 80 keep two
+// CTAs of 384 threads (17408 x 6144: 119 us; with the 87 the compiler takes unasked, one CTA, 168).
+template <typename TX, typename TY, int C, int WARPS>
+__global__ void __maxnreg__(WARPS == 32 ? 64 : C == 1 ? 80 : 128) rms_f8_kernel(const RmsArgs p) {
+  __shared__ alignas(16) float part[2][WARPS];  // the warps' sums of squares, zeros for warps that do not exist
   grid_dep_launch();
   grid_dep_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  const long long m = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool one_warp = blockDim.x == 32;
   constexpr bool kAdd = !std::is_same<TY, None>::value;
-  float2 v[C][kPiece / 2];
-  float2 ss2 = both(0.0f);
+  using Y = std::conditional_t<kAdd, TY, TX>;
+  Raw<TX> x;
+  Raw<Y> y;
+  auto fetch = [&](long long m, int c) {
+    const int at = (threadIdx.x + c * blockDim.x) * kPiece, n = p.D - at;
+    if (n <= 0 || m >= p.M) return;
+    x.load(static_cast<const TX *>(p.x) + m * p.x_stride + at, n, p.x_align);
+    if constexpr (kAdd) y.load(static_cast<const TY *>(p.y) + m * p.y_stride + at, n, p.y_align);
+  };
+  auto gain_of = [&](int c, float2 (&g)[kPiece / 2]) {
+    const int at = (threadIdx.x + c * blockDim.x) * kPiece, n = p.D - at;
+    if (n <= 0) return;
+    if (p.w_dtype == kDtypeF32) read_gain<float>(g, p.w, at, n, p.w_align);
+    else if (p.w_dtype == kDtypeBf16) read_gain<__nv_bfloat16>(g, p.w, at, n, p.w_align);
+    else read_gain<__half>(g, p.w, at, n, p.w_align);
+  };
+  if (!one_warp) {
+    for (int i = threadIdx.x; i < 2 * WARPS; i += blockDim.x) part[0][i] = 0.0f;  // blockDim.y is 1
+    __syncthreads();
+  }
+  float2 gain[kPiece / 2] = {};
+  const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
+  long long m = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if constexpr (C == 1) {
+    fetch(m, 0);
+    gain_of(0, gain);
+  }
+  for (int turn = 0; m < p.M; m += step, turn ^= 1) {  // the same for all threads of a row, and rows only meet a barrier alone
+    float2 v[C][kPiece / 2];
+    float2 ss2 = both(0.0f);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = (tid + c * blockDim.x) * kPiece, n = p.D - at;
-    if (n > 0) {
-      Raw<TX> x;
-      x.load(static_cast<const TX *>(p.x) + m * p.x_stride + at, n, true);
-      if constexpr (kAdd) {
-        Raw<TY> y;
-        y.load(static_cast<const TY *>(p.y) + m * p.y_stride + at, n, true);
-#pragma unroll
-        for (int i = 0; i < kPiece / 2; ++i) x.set(i, __fadd2_rn(x.get(i), y.get(i)));
-        x.store(static_cast<TX *>(p.res) + m * p.res_stride + at, n);
-      }
-#pragma unroll
-      for (int i = 0; i < kPiece / 2; ++i) v[c][i] = x.get(i);
-    } else {
+    for (int c = 0; c < C; ++c) {
+      const int at = (threadIdx.x + c * blockDim.x) * kPiece, n = p.D - at;
+      if constexpr (C > 1) fetch(m, c);
 #pragma unroll
       for (int i = 0; i < kPiece / 2; ++i) v[c][i] = both(0.0f);
+      if (n > 0) {
+        if constexpr (kAdd) {
+#pragma unroll
+          for (int i = 0; i < kPiece / 2; ++i) x.set(i, __fadd2_rn(x.get(i), y.get(i)));
+          x.store(static_cast<TX *>(p.res) + m * p.res_stride + at, n, p.res_align);
+        }
+#pragma unroll
+        for (int i = 0; i < kPiece / 2; ++i) v[c][i] = x.get(i);
+      }
+#pragma unroll
+      for (int i = 0; i < kPiece / 2; ++i) ss2 = __ffma2_rn(v[c][i], v[c][i], ss2);
     }
+    if constexpr (C == 1) fetch(m + step, 0);
+    float ss = __fadd_rn(ss2.x, ss2.y);
 #pragma unroll
-    for (int i = 0; i < kPiece / 2; ++i) ss2 = __ffma2_rn(v[c][i], v[c][i], ss2);
-  }
-  float ss = __fadd_rn(ss2.x, ss2.y);
+    for (int s = 16; s > 0; s >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, s));
+    if (!one_warp) {  // two sets of partial sums: the next row's cannot meet a warp that still reads this row's
+      if (lane == 0) part[turn][warp] = ss;
+      __syncthreads();
+      float2 sum = both(0.0f);
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, s));
-  if (warps > 1) {
-    if (lane == 0) part[warp] = ss;
-    __syncthreads();
-    ss = part[0];
-    for (int i = 1; i < warps; ++i) ss = __fadd_rn(ss, part[i]);
-  }
-  const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int piece = tid + c * blockDim.x, at = piece * kPiece, n = p.D - at;
-    if (n > 0) {
-      if (p.w_dtype == kDtypeF32) scale_by<float>(v[c], p.w, at, n, inv);
-      else if (p.w_dtype == kDtypeBf16) scale_by<__nv_bfloat16>(v[c], p.w, at, n, inv);
-      else scale_by<__half>(v[c], p.w, at, n, inv);
+      for (int i = 0; i < WARPS / 4; ++i) {
+        const float4 q = reinterpret_cast<const float4 *>(part[turn])[i];
+        sum = __fadd2_rn(sum, __fadd2_rn(make_float2(q.x, q.y), make_float2(q.z, q.w)));
+      }
+      ss = __fadd_rn(sum.x, sum.y);
     }
-    const int group = piece >> 3;
-    encode_piece(v[c], n, p.out + m * p.out_stride + at, p.sa + group * p.sa_stride + m,
-                 (piece & 7) == 0 && group * kGroup < p.D);
+    const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.D)), p.eps));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int piece = threadIdx.x + c * blockDim.x, at = piece * kPiece, n = p.D - at;
+      if constexpr (C > 1) gain_of(c, gain);
+#pragma unroll
+      for (int i = 0; i < kPiece / 2; ++i) v[c][i] = __fmul2_rn(__fmul2_rn(v[c][i], both(inv)), gain[i]);
+      const int group = piece >> 3;
+      encode_piece(v[c], n, p.out + m * p.out_stride + at, p.sa + group * p.sa_stride + m,
+                   (piece & 7) == 0 && group * kGroup < p.D);
+    }
   }
 }
 
@@ -269,24 +319,52 @@ cudaError_t launch(F *kernel, dim3 grid, dim3 threads, bool overlap, cudaStream_
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename TX, typename TY>
-cudaError_t launch_rms(const RmsArgs &a, int M, bool overlap, cudaStream_t stream) {
-  const int pieces = (a.D + kGroup - 1) / kGroup * (kGroup / kPiece);
-  const int c = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
-  const unsigned threads = ((pieces + c - 1) / c + 31) / 32 * 32;
-  switch (c) {
-    case 1: return launch(rms_f8_kernel<TX, TY, 1>, dim3(M), dim3(threads), overlap, stream, a);
-    case 2: return launch(rms_f8_kernel<TX, TY, 2>, dim3(M), dim3(threads), overlap, stream, a);
-    default: return launch(rms_f8_kernel<TX, TY, 4>, dim3(M), dim3(threads), overlap, stream, a);
+// 32, 16 or 1: the boundary on which every row of a tensor starts
+int boundary(const void *p, long long row_bytes) {
+  const unsigned long long bits = reinterpret_cast<uintptr_t>(p) | static_cast<unsigned long long>(row_bytes);
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 1;
+}
+
+// CTAs of this kernel that an SM holds at once, asked once per CTA size.
+template <typename TX, typename TY, int C, int WARPS>
+int rms_resident(unsigned threads) {
+  static std::atomic<int> known[WARPS + 1];
+  int n = known[threads / 32].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rms_f8_kernel<TX, TY, C, WARPS>, static_cast<int>(threads), 0) != cudaSuccess || n < 1) n = 1;
+    known[threads / 32].store(n, std::memory_order_relaxed);
   }
+  return n;
+}
+
+template <typename TX, typename TY, int C, int WARPS>
+cudaError_t launch_rms_c(RmsArgs a, int pieces, int sms, bool overlap, cudaStream_t stream) {
+  const unsigned tx = ((pieces + C - 1) / C + 31) / 32 * 32;
+  const unsigned ty = tx == 32 ? 4 : 1;  // rows of up to 512 channels: a warp each, four to a CTA
+  a.x_align = boundary(a.x, a.x_stride * sizeof(TX));
+  a.w_align = boundary(a.w, 0);
+  if constexpr (!std::is_same<TY, None>::value) {
+    a.y_align = boundary(a.y, a.y_stride * sizeof(TY));
+    a.res_align = boundary(a.res, a.res_stride * sizeof(TX));
+  }
+  const int resident = sms * rms_resident<TX, TY, C, WARPS>(tx * ty), wanted = (a.M - 1) / static_cast<int>(ty) + 1;
+  return launch(rms_f8_kernel<TX, TY, C, WARPS>, dim3(wanted < resident ? wanted : resident), dim3(tx, ty), overlap, stream, a);
+}
+
+template <typename TX, typename TY>
+cudaError_t launch_rms(const RmsArgs &a, int sms, bool overlap, cudaStream_t stream) {
+  const int pieces = (a.D + kGroup - 1) / kGroup * (kGroup / kPiece);
+  if (pieces <= 512) return launch_rms_c<TX, TY, 1, 16>(a, pieces, sms, overlap, stream);
+  if (pieces <= 1024) return launch_rms_c<TX, TY, 1, 32>(a, pieces, sms, overlap, stream);
+  return launch_rms_c<TX, TY, 4, 16>(a, pieces, sms, overlap, stream);
 }
 
 template <typename TX>
-cudaError_t launch_rms_y(const RmsArgs &a, int y_dtype, int M, bool overlap, cudaStream_t stream) {
-  if (!a.y) return launch_rms<TX, None>(a, M, overlap, stream);
-  if (y_dtype == kDtypeF32) return launch_rms<TX, float>(a, M, overlap, stream);
-  if (y_dtype == kDtypeF16) return launch_rms<TX, __half>(a, M, overlap, stream);
-  return launch_rms<TX, __nv_bfloat16>(a, M, overlap, stream);
+cudaError_t launch_rms_y(const RmsArgs &a, int y_dtype, int sms, bool overlap, cudaStream_t stream) {
+  if (!a.y) return launch_rms<TX, None>(a, sms, overlap, stream);
+  if (y_dtype == kDtypeF32) return launch_rms<TX, float>(a, sms, overlap, stream);
+  if (y_dtype == kDtypeF16) return launch_rms<TX, __half>(a, sms, overlap, stream);
+  return launch_rms<TX, __nv_bfloat16>(a, sms, overlap, stream);
 }
 
 template <typename T>
@@ -294,7 +372,8 @@ cudaError_t launch_quant(const QuantF8Launch &q, bool overlap, cudaStream_t stre
   QuantArgs a;
   a.x = q.x; a.out = static_cast<uint8_t *>(q.out); a.sa = q.sa;
   a.x_stride = q.x_stride; a.out_stride = q.out_stride; a.sa_stride = q.sa_stride; a.M = q.M; a.D = q.D;
-  a.gate_vec = (static_cast<long long>(q.D) * sizeof(T)) % 16 == 0;
+  a.x_align = boundary(q.x, q.x_stride * sizeof(T));
+  a.gate_align = boundary(static_cast<const T *>(q.x) + q.D, q.x_stride * sizeof(T));
   // About 256 threads: parts of a row of equal length, or several short rows. Whole warps, whole groups of eight lanes.
   const int pieces = (q.D + kGroup - 1) / kGroup * (kGroup / kPiece);
   const int parts = (pieces + 255) / 256;
@@ -320,14 +399,14 @@ cudaError_t launch_quant_f8(const QuantF8Launch &q, bool overlap, cudaStream_t s
   return launch_quant<__nv_bfloat16>(q, overlap, stream);
 }
 
-cudaError_t launch_rms_f8(const RmsF8Launch &r, bool overlap, cudaStream_t stream) {
+cudaError_t launch_rms_f8(const RmsF8Launch &r, int sms, bool overlap, cudaStream_t stream) {
   RmsArgs a;
   a.x = r.x; a.y = r.y; a.w = r.w; a.res = r.res; a.out = static_cast<uint8_t *>(r.out); a.sa = r.sa;
   a.x_stride = r.x_stride; a.y_stride = r.y_stride; a.res_stride = r.res_stride; a.out_stride = r.out_stride;
-  a.sa_stride = r.sa_stride; a.D = r.D; a.w_dtype = r.w_dtype; a.eps = r.eps;
-  if (r.x_dtype == kDtypeF32) return launch_rms_y<float>(a, r.y_dtype, r.M, overlap, stream);
-  if (r.x_dtype == kDtypeF16) return launch_rms_y<__half>(a, r.y_dtype, r.M, overlap, stream);
-  return launch_rms_y<__nv_bfloat16>(a, r.y_dtype, r.M, overlap, stream);
+  a.sa_stride = r.sa_stride; a.M = r.M; a.D = r.D; a.w_dtype = r.w_dtype; a.eps = r.eps;
+  if (r.x_dtype == kDtypeF32) return launch_rms_y<float>(a, r.y_dtype, sms, overlap, stream);
+  if (r.x_dtype == kDtypeF16) return launch_rms_y<__half>(a, r.y_dtype, sms, overlap, stream);
+  return launch_rms_y<__nv_bfloat16>(a, r.y_dtype, sms, overlap, stream);
 }
 
 }  // namespace h3b
