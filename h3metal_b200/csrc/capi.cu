@@ -835,9 +835,10 @@ static bool rows_aligned(const void *p, int64_t stride, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * size) % 16 == 0;
 }
 
-int h3b_quant_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, void *out, int64_t out_stride, float *sa,
-                 int64_t sa_stride, int M, int D, int mode) {
+int h3b_quant_f8(h3b_ctx *ctx, const h3b_quant_f8_args *args) {
   if (!ctx) return fail("null context");
+  if (!args) return fail("quant_f8: null argument block");
+  const auto &[x, x_stride, out, out_stride, sa, sa_stride, x_dtype, M, D, mode] = *args;
   if (!x || !out || !sa) return fail("quant_f8: null tensor argument");
   if (M <= 0 || D <= 0) return fail("quant_f8: M and D must be positive");
   if (mode != 0 && mode != 1) return fail("quant_f8: mode must be 0 or 1");
@@ -856,10 +857,11 @@ int h3b_quant_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, voi
   return ctx->after_launch("quant_f8 launch", h3b::launch_quant_f8(q, ctx->overlap != 0 && !ctx->profile, ctx->stream));
 }
 
-int h3b_rms_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, const void *y, int y_dtype, int64_t y_stride,
-               void *res, int64_t res_stride, const void *w, int w_dtype, void *out, int64_t out_stride, float *sa,
-               int64_t sa_stride, int M, int D, float eps) {
+int h3b_rms_f8(h3b_ctx *ctx, const h3b_rms_f8_args *args) {
   if (!ctx) return fail("null context");
+  if (!args) return fail("rms_f8: null argument block");
+  const auto &[x, x_stride, y, y_stride, res, res_stride, w, out, out_stride, sa, sa_stride, x_dtype, y_dtype, w_dtype, M, D,
+               eps] = *args;
   if (!x || !w || !out || !sa) return fail("rms_f8: null tensor argument");
   if ((y != nullptr) != (res != nullptr)) return fail("rms_f8: y and res go together");
   if (M <= 0 || D <= 0) return fail("rms_f8: M and D must be positive");
@@ -882,10 +884,10 @@ int h3b_rms_f8(h3b_ctx *ctx, const void *x, int x_dtype, int64_t x_stride, const
   return ctx->after_launch("rms_f8 launch", h3b::launch_rms_f8(r, ctx->prop.multiProcessorCount, ctx->overlap != 0 && !ctx->profile, ctx->stream));
 }
 
-int h3b_gemm_f8(h3b_ctx *ctx, const void *A, int64_t a_stride, const float *sa, int64_t sa_stride, const void *W,
-                int64_t w_stride, const float *sw, int64_t sw_stride, const float *bias, void *C, int c_dtype,
-                int64_t c_stride, int M, int N, int K) {
+int h3b_gemm_f8(h3b_ctx *ctx, const h3b_gemm_f8_args *args) {
   if (!ctx) return fail("null context");
+  if (!args) return fail("gemm_f8: null argument block");
+  const auto &[A, a_stride, sa, sa_stride, W, w_stride, sw, sw_stride, bias, C, c_stride, c_dtype, M, N, K] = *args;
   if (!A || !sa || !W || !sw || !C) return fail("gemm_f8: null tensor argument");
   if (M <= 0 || N <= 0 || K <= 0) return fail("gemm_f8: M, N and K must be positive");
   if (!float_size(c_dtype)) return fail("gemm_f8: output type must be bf16, f16 or f32");

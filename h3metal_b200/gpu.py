@@ -86,9 +86,9 @@ def _signatures():
         "h3b_reduce_dequant_low": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, i64, ctypes.POINTER(vp), i32, i32, i64, i32,
                                          i32, i32, vp, vp, i64]),
         "h3b_reduce_dequant_gated": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, vp, i64]),
-        "h3b_rms_f8": (i32, [vp, vp, i32, i64, vp, i32, i64, vp, i64, vp, i32, vp, i64, vp, i64, i32, i32, ctypes.c_float]),
-        "h3b_quant_f8": (i32, [vp, vp, i32, i64, vp, i64, vp, i64, i32, i32, i32]),
-        "h3b_gemm_f8": (i32, [vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i32, i32, i32]),
+        "h3b_rms_f8": (i32, [vp, cp]),
+        "h3b_quant_f8": (i32, [vp, cp]),
+        "h3b_gemm_f8": (i32, [vp, cp]),
         "h3b_gemm_tile_n": (i32, [vp, i32, i32]),
         "h3b_gemm_set_policy": (i32, [vp, i32, i32, i32]),
         "h3b_gemm_set_store_mode": (i32, [vp, i32]),
@@ -101,6 +101,12 @@ def _signatures():
         "h3b_profile_take": (i32, [vp, ctypes.POINTER(dbl), i32]),
         "h3b_launch_count": (u64, [vp]),
     }
+
+
+# the argument blocks of the block-scaled calls (h3b_rms_f8_args, h3b_quant_f8_args, h3b_gemm_f8_args), native alignment
+_RMS_F8 = struct.Struct("@PqPqPqPPqPqiiiiif")
+_QUANT_F8 = struct.Struct("@PqPqPqiiii")
+_GEMM_F8 = struct.Struct("@PqPqPqPqPPqiiii")
 
 
 def _load():
@@ -160,14 +166,14 @@ class Tensor:
     shape: tuple
     dtype: str
     strides: tuple = field(default=None)  # in elements; None = contiguous
+    numel: int = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self):
+        self.numel = math.prod(self.shape)
 
     @property
     def nbytes(self) -> int:
         return int(math.prod(self.shape) * _SIZE[self.dtype])
-
-    @property
-    def numel(self) -> int:
-        return math.prod(self.shape)
 
     @property
     def ptr(self) -> int:
@@ -332,26 +338,29 @@ class Gpu:
     def rms_f8_native(self, x: Tensor, x_stride: int, y: Tensor | None, y_stride: int, res: Tensor | None, res_stride: int,
                       w: Tensor, out: Tensor, out_stride: int, sa: Tensor, sa_stride: int, M: int, D: int, eps: float,
                       name: str = "rms_f8"):
-        self._check(lib().h3b_rms_f8(self.ctx, x.ptr, _ABI_DTYPE[x.dtype], x_stride, y.ptr if y is not None else None,
-                                      _ABI_DTYPE[y.dtype] if y is not None else 0, y_stride,
-                                      res.ptr if res is not None else None, res_stride, w.ptr, _ABI_DTYPE[w.dtype], out.ptr,
-                                      out_stride, sa.ptr, sa_stride, M, D, eps))
+        block = _RMS_F8.pack(x.ptr, x_stride, y.ptr if y is not None else 0, y_stride, res.ptr if res is not None else 0,
+                             res_stride, w.ptr, out.ptr, out_stride, sa.ptr, sa_stride, _ABI_DTYPE[x.dtype],
+                             _ABI_DTYPE[y.dtype] if y is not None else 0, _ABI_DTYPE[w.dtype], M, D, eps)
+        if lib().h3b_rms_f8(self.ctx, block):
+            raise GpuError(_err())
         if self._profile:
             self.names.append(name)
 
     def quant_f8_native(self, x: Tensor, x_stride: int, out: Tensor, out_stride: int, sa: Tensor, sa_stride: int, M: int,
                         D: int, mode: int, name: str = "quant_f8"):
-        self._check(lib().h3b_quant_f8(self.ctx, x.ptr, _ABI_DTYPE[x.dtype], x_stride, out.ptr, out_stride, sa.ptr,
-                                        sa_stride, M, D, mode))
+        if lib().h3b_quant_f8(self.ctx, _QUANT_F8.pack(x.ptr, x_stride, out.ptr, out_stride, sa.ptr, sa_stride,
+                                                       _ABI_DTYPE[x.dtype], M, D, mode)):
+            raise GpuError(_err())
         if self._profile:
             self.names.append(name)
 
     def gemm_f8_native(self, a: Tensor, a_stride: int, sa: Tensor, sa_stride: int, w: Tensor, w_stride: int, sw: Tensor,
                        sw_stride: int, bias: Tensor | None, out: Tensor, c_stride: int, M: int, N: int, K: int,
                        name: str = "gemm(f8)"):
-        self._check(lib().h3b_gemm_f8(self.ctx, a.ptr, a_stride, sa.ptr, sa_stride, w.ptr, w_stride, sw.ptr, sw_stride,
-                                       bias.ptr if bias is not None else None, out.ptr, _ABI_DTYPE[out.dtype], c_stride, M,
-                                       N, K))
+        block = _GEMM_F8.pack(a.ptr, a_stride, sa.ptr, sa_stride, w.ptr, w_stride, sw.ptr, sw_stride,
+                              bias.ptr if bias is not None else 0, out.ptr, c_stride, _ABI_DTYPE[out.dtype], M, N, K)
+        if lib().h3b_gemm_f8(self.ctx, block):
+            raise GpuError(_err())
         if self._profile:
             self.names.append(name)
 

@@ -282,12 +282,13 @@ def rot_q8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor | None, M: int, D: int, 
 _FLOATS = ("bf16", "f16", "f32")
 
 
-def _rows(what: str, t: Tensor, types, rows: int, cols: int, stride: int):
-    """Refuses a tensor of another type, a stride shorter than its rows, and a buffer that ends before the last of them."""
-    if t.dtype not in types:
-        raise ValueError(f"{what}: type {t.dtype}, not {' / '.join(types)}")
-    if stride < cols or (rows - 1) * stride + cols > t.numel:
-        raise ValueError(f"{what}: {t.shape} does not hold {rows} rows of {cols} values {stride} apart")
+def _holds(t: Tensor, types, rows: int, cols: int, stride: int) -> bool:
+    """The tensor is of one of these types, its stride covers its rows, and its buffer does not end before the last of them."""
+    return t.dtype in types and stride >= cols and (rows - 1) * stride + cols <= t.numel
+
+
+def _refuse(what: str, t: Tensor, types, rows: int, cols: int, stride: int):
+    raise ValueError(f"{what}: {t.dtype} {t.shape} does not hold {rows} rows of {cols} {' / '.join(types)} values {stride} apart")
 
 
 def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: int, *, eps: float, y: Tensor | None = None,
@@ -299,10 +300,14 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
     if M <= 0 or D <= 0:
         raise ValueError("rms_f8: M and D must be positive")
     x_stride, out_stride, sa_stride = x_stride or D, out_stride or f8_stride(D), sa_stride or M
-    _rows("rms_f8 x", x, _FLOATS, M, D, x_stride)
-    _rows("rms_f8 w", w, _FLOATS, 1, D, D)
-    _rows("rms_f8 out", out, ("f8",), M, D, out_stride)
-    _rows("rms_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
+    if not _holds(x, _FLOATS, M, D, x_stride):
+        _refuse("rms_f8 x", x, _FLOATS, M, D, x_stride)
+    if not _holds(w, _FLOATS, 1, D, D):
+        _refuse("rms_f8 w", w, _FLOATS, 1, D, D)
+    if not _holds(out, ("f8",), M, D, out_stride):
+        _refuse("rms_f8 out", out, ("f8",), M, D, out_stride)
+    if not _holds(sa, ("f32",), -(-D // F8_GROUP), M, sa_stride):
+        _refuse("rms_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
     if y is None:
         if res is not None:
             raise ValueError("rms_f8: res is where x + y goes: it needs y")
@@ -311,8 +316,10 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
         if res is None:
             res, res_stride = x, res_stride or x_stride
         y_stride, res_stride = y_stride or D, res_stride or D
-        _rows("rms_f8 y", y, _FLOATS, M, D, y_stride)
-        _rows("rms_f8 res", res, (x.dtype,), M, D, res_stride)
+        if not _holds(y, _FLOATS, M, D, y_stride):
+            _refuse("rms_f8 y", y, _FLOATS, M, D, y_stride)
+        if not _holds(res, (x.dtype,), M, D, res_stride):
+            _refuse("rms_f8 res", res, (x.dtype,), M, D, res_stride)
     gpu.rms_f8_native(x, x_stride, y, y_stride, res, res_stride, w, out, out_stride, sa, sa_stride, M, D, eps,
                       name=f"rms_f8({D}{',add' if y is not None else ''})" if gpu._profile else "")
 
@@ -325,9 +332,12 @@ def quant_f8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor, M: int, D: int, *, sw
         raise ValueError("quant_f8: M and D must be positive")
     wide = 2 * D if swiglu else D
     x_stride, out_stride, sa_stride = x_stride or wide, out_stride or f8_stride(D), sa_stride or M
-    _rows("quant_f8 x", x, _FLOATS, M, wide, x_stride)
-    _rows("quant_f8 out", out, ("f8",), M, D, out_stride)
-    _rows("quant_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
+    if not _holds(x, _FLOATS, M, wide, x_stride):
+        _refuse("quant_f8 x", x, _FLOATS, M, wide, x_stride)
+    if not _holds(out, ("f8",), M, D, out_stride):
+        _refuse("quant_f8 out", out, ("f8",), M, D, out_stride)
+    if not _holds(sa, ("f32",), -(-D // F8_GROUP), M, sa_stride):
+        _refuse("quant_f8 sa", sa, ("f32",), -(-D // F8_GROUP), M, sa_stride)
     gpu.quant_f8_native(x, x_stride, out, out_stride, sa, sa_stride, M, D, 1 if swiglu else 0,
                         name=f"quant_f8({D}{',swiglu' if swiglu else ''})" if gpu._profile else "")
 
@@ -347,12 +357,18 @@ def gemm_f8(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor
         raise ValueError("gemm_f8: M, N and K must be positive")
     groups = -(-K // F8_GROUP)
     a_stride, sa_stride, c_stride, w_stride = a_stride or f8_stride(K), sa_stride or M, c_stride or N, wt.ws or f8_stride(K)
-    _rows("gemm_f8 a", a, ("f8",), M, K, a_stride)
-    _rows("gemm_f8 sa", sa, ("f32",), groups, M, sa_stride)
-    _rows("gemm_f8 weight", wt.w, ("f8",), N, K, w_stride)
-    _rows("gemm_f8 weight scales", wt.sw, ("f32",), -(-N // F8_GROUP), groups, groups)
-    _rows("gemm_f8 out", out, _FLOATS, M, N, c_stride)
+    if not _holds(a, ("f8",), M, K, a_stride):
+        _refuse("gemm_f8 a", a, ("f8",), M, K, a_stride)
+    if not _holds(sa, ("f32",), groups, M, sa_stride):
+        _refuse("gemm_f8 sa", sa, ("f32",), groups, M, sa_stride)
+    if not _holds(wt.w, ("f8",), N, K, w_stride):
+        _refuse("gemm_f8 weight", wt.w, ("f8",), N, K, w_stride)
+    if not _holds(wt.sw, ("f32",), -(-N // F8_GROUP), groups, groups):
+        _refuse("gemm_f8 weight scales", wt.sw, ("f32",), -(-N // F8_GROUP), groups, groups)
+    if not _holds(out, _FLOATS, M, N, c_stride):
+        _refuse("gemm_f8 out", out, _FLOATS, M, N, c_stride)
     if wt.bias is not None:
-        _rows("gemm_f8 bias", wt.bias, ("f32",), 1, N, N)
+        if not _holds(wt.bias, ("f32",), 1, N, N):
+            _refuse("gemm_f8 bias", wt.bias, ("f32",), 1, N, N)
     gpu.gemm_f8_native(a, a_stride, sa, sa_stride, wt.w, w_stride, wt.sw, groups, wt.bias, out, c_stride, M, N, K,
                        name=f"gemm(f8,{K}->{N})" if gpu._profile else "")
