@@ -27,7 +27,6 @@ using namespace gemm;
 
 constexpr int kF8BN = 256;
 constexpr int kF8Stage = kABytes + 128 * kBKBytes;  // 32 KB: this CTA's rows of A and its half of W
-constexpr int kF8Stages = 5;
 constexpr int kF8EpiWarps = 8;
 constexpr int kF8Cols = kF8BN / (kF8EpiWarps / 4);  // columns per epilogue thread: 128, those of one weight block
 constexpr int kF8Threads = 128 + 32 * kF8EpiWarps;
@@ -35,7 +34,18 @@ constexpr int kF8Threads = 128 + 32 * kF8EpiWarps;
 // given. Neither side spills with these; 56 and 224 make the issuing warps spill and cost 6 % of the whole product.
 constexpr int kF8RegsIssue = 104, kF8RegsEpi = 200;
 constexpr int kF8OutWarp = 2 * kOutPanel;           // a warp's 32 rows x 128 two-byte columns
-constexpr int kF8OutBytes = kF8EpiWarps * kF8OutWarp;
+constexpr int kF8MailWarp = 32 * 128 * 4;           // a warp's 32 x 128 fp32 sums
+
+// SPLIT 1: a pair has the whole of K, eight warps stage results. SPLIT 2: two pairs of a cluster have half of K each for ONE tile
+// per cluster; four warps of each stage results and receive the other pair's sums.
+template <int SPLIT> struct PairShape {
+  static constexpr int kStages = SPLIT == 1 ? 5 : 4;
+  static constexpr int kMailOff = kStages * kF8Stage;
+  static constexpr int kOutOff = kMailOff + (SPLIT == 1 ? 0 : 4 * kF8MailWarp);
+  static constexpr int kBarsOff = kOutOff + (SPLIT == 1 ? 8 : 4) * kF8OutWarp;
+  static constexpr size_t kSmem = 1024 + kBarsOff + kBarrierBytes;
+  static_assert(kSmem <= 232448, "ring, mail and staging share 227 KB");
+};
 
 // acc += p * s for 16 columns, two at a time
 __device__ __forceinline__ void scale_add16(const uint32_t (&p)[16], float2 s2, float2 *acc) {
@@ -74,31 +84,34 @@ __device__ __forceinline__ void store_chunk(const GemmF8Launch &g, float *buf, i
 }
 
 // STAGED: 16-bit results by TMA (g.map_c). A kernel of its own, because the other way out costs the main loop registers.
-template <bool STAGED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kF8Threads, 1)
+template <bool STAGED, int SPLIT>
+__global__ void __cluster_dims__(2 * SPLIT, 1, 1) __launch_bounds__(kF8Threads, 1)
 gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t *base_ptr = smem_raw + (base - raw_addr);
-  // [ring: 5 x 32 KB][staging of results: 64 KB][barriers 256 B]
-  constexpr int stages = kF8Stages;
-  constexpr uint32_t out_off = stages * kF8Stage;
-  constexpr uint32_t bars_off = out_off + kF8OutBytes;
+  // [ring][mail: 64 KB, split only][staging of results][barriers 256 B]
+  using P = PairShape<SPLIT>;
+  constexpr int stages = P::kStages;
+  constexpr uint32_t bars_off = P::kBarsOff;
   const uint32_t bars = base + bars_off;
   auto full_bar = [&](int i) { return bars + 8u * i; };
   auto done_bar = [&](int i) { return bars + 64u + 8u * i; };
-  auto acc_empty_bar = [&](int i) { return bars + 144u + 8u * i; };
+  auto acc_empty_bar = [&](int i) { return bars + 128u + 8u * i; };
   volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(base_ptr + bars_off + 176);
   volatile int *cta_abort = reinterpret_cast<volatile int *>(base_ptr + bars_off + 180);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_cta_rank();
+  const uint32_t cta = cluster_cta_rank(), rank = cta & 1u;  // rank in the pair
+  const int pair = SPLIT == 1 ? 0 : static_cast<int>(cta >> 1);
+  const uint32_t leader_cta = cta & ~1u;
   const bool leader = rank == 0;
   const int n_tiles = (g.N + kF8BN - 1) / kF8BN;
   const int num_tiles = g.m_tiles * n_tiles;
-  const int groups = (g.K + kBKBytes - 1) / kBKBytes;
-  const int first_tile = cluster_id_x(), tile_step = cluster_count_x();
+  const int all_groups = (g.K + kBKBytes - 1) / kBKBytes;
+  const int g_begin = all_groups * pair / SPLIT, groups = all_groups * (pair + 1) / SPLIT - g_begin;
+  const int first_tile = cluster_id_x(), tile_step = SPLIT == 1 ? static_cast<int>(cluster_count_x()) : num_tiles;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_descriptor(&g.map_a);
@@ -129,7 +142,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
       if (lane == 0) {
         RingPos pos;
         uint32_t filled = 0;  // stages filled so far, saturating at `stages` (for the wind-down)
-        const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
+        const uint32_t leader_full0 = map_to_cta(full_bar(0), leader_cta);
         bool ok = true;
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
           const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
@@ -142,8 +155,8 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
             if (leader) mbar_arrive_expect_tx(full_bar(s), 2u * kF8Stage);
             const uint32_t leader_full = leader_full0 + 8u * s;
             const uint32_t dst = base + s * kF8Stage;
-            tma_load_2d_pair(dst, &g.map_a, leader_full, kb * kBKBytes, m0);
-            tma_load_2d_pair(dst + kABytes, &g.map_w, leader_full, kb * kBKBytes, n0);
+            tma_load_2d_pair(dst, &g.map_a, leader_full, (g_begin + kb) * kBKBytes, m0);
+            tma_load_2d_pair(dst + kABytes, &g.map_w, leader_full, (g_begin + kb) * kBKBytes, n0);
             pos.advance(stages);
             filled += filled < static_cast<uint32_t>(stages);
           }
@@ -179,19 +192,24 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
             const uint32_t d = tmem_base + buf.s * kF8BN;
 #pragma unroll
             for (int k = 0; k < kBKBytes / 32; ++k) umma_f8_pair(d, ad + 2u * k, bd + 2u * k, idesc, k ? 1u : 0u);
-            umma_commit_pair(done_bar(s), 3);  // the stage may be refilled, the accumulator read
+            umma_commit_pair(done_bar(s), static_cast<uint16_t>(3u << leader_cta));  // the stage may be refilled, the accumulator read
             pos.advance(stages);
             buf.advance(2);
           }
         }
       }
     }
+    if (SPLIT > 1) {  // the barrier between the pairs' sums (see the epilogue)
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8RegsEpi));
     const int quarter = warp & 3, part = (warp - 4) >> 2;
     const int row = quarter * 32 + lane;
     const int n_blocks = (g.N + 127) / 128;
-    const uint32_t leader_acc_empty0 = map_to_cta(acc_empty_bar(0), 0);
+    const uint32_t leader_acc_empty0 = map_to_cta(acc_empty_bar(0), leader_cta);
     RingPos pos;
     uint32_t buf = 0;
     bool ok = true;
@@ -205,13 +223,14 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
 #pragma unroll
       for (int j = 0; j < kF8Cols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
       // the next group's scales are fetched while this group's are waited for and used
-      float a_s = __ldg(g.sa + m_s), w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride);
+      float a_s = __ldg(g.sa + static_cast<size_t>(g_begin) * g.sa_stride + m_s);
+      float w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin);
 #pragma unroll 1
       for (int kb = 0; kb < groups; ++kb) {
         const float s = __fmul_rn(a_s, w_s);
         if (kb + 1 < groups) {
-          a_s = __ldg(g.sa + static_cast<size_t>(kb + 1) * g.sa_stride + m_s);
-          w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + kb + 1);
+          a_s = __ldg(g.sa + static_cast<size_t>(g_begin + kb + 1) * g.sa_stride + m_s);
+          w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin + kb + 1);
         }
         ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
         ok = __all_sync(0xFFFFFFFFu, ok);  // a warp gives up as a whole
@@ -236,6 +255,29 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
         pos.advance(stages);
         buf ^= 1u;
       }
+      if constexpr (SPLIT > 1) {
+        // Each pair finishes one column half: the warps of the other half leave their sums with the same warp quarter of the
+        // other pair's CTA with the same rows, 16 bytes per lane at [piece of four columns][lane]. A cluster has one tile, so
+        // the two barriers of the cluster, here and at the end, are all it takes; a warp that gave up meets them too.
+        if (ok && part != pair) {
+          const uint32_t dst = map_to_cta(base + P::kMailOff + quarter * kF8MailWarp + lane * 16, cta ^ 2u);
+#pragma unroll
+          for (int q = 0; q < kF8Cols / 4; ++q)
+            st_cluster_v4(dst + q * 512, acc[2 * q].x, acc[2 * q].y, acc[2 * q + 1].x, acc[2 * q + 1].y);
+        }
+        cluster_arrive();
+        cluster_wait();
+        if (part != pair) break;
+        if (ok) {
+          const float4 *mail = reinterpret_cast<const float4 *>(base_ptr + P::kMailOff + quarter * kF8MailWarp) + lane;
+#pragma unroll
+          for (int q = 0; q < kF8Cols / 4; ++q) {
+            const float4 x = mail[q * 32];
+            acc[2 * q] = __fadd2_rn(acc[2 * q], make_float2(x.x, x.y));
+            acc[2 * q + 1] = __fadd2_rn(acc[2 * q + 1], make_float2(x.z, x.w));
+          }
+        }
+      }
       if (!ok) break;
       float bias[kF8Cols / 32];
 #pragma unroll
@@ -243,8 +285,9 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
         const int n = n0 + j * 32 + lane;
         bias[j] = g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
       }
-      uint8_t *out_buf = base_ptr + out_off + (part * 4 + quarter) * kF8OutWarp;
-      const uint32_t out_addr = base + out_off + (part * 4 + quarter) * kF8OutWarp;
+      const int out_warp = SPLIT == 1 ? part * 4 + quarter : quarter;
+      uint8_t *out_buf = base_ptr + P::kOutOff + out_warp * kF8OutWarp;
+      const uint32_t out_addr = base + P::kOutOff + out_warp * kF8OutWarp;
       if constexpr (STAGED) {  // the panels of the tile before must have been read out of shared memory
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
@@ -295,41 +338,50 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
   }
 }
 
-constexpr size_t kF8Smem = 1024 + static_cast<size_t>(kF8Stages) * kF8Stage + kF8OutBytes + kBarrierBytes;
-static_assert(kF8Smem <= 232448, "ring and staging share 227 KB");
-
-}  // namespace
-
-cudaError_t gemm_f8_pair_configure(int *clusters) {
-  *clusters = 0;
-  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+template <int SPLIT>
+cudaError_t configure(int *clusters) {
+  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel<true, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairShape<SPLIT>::kSmem);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(gemm_f8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+  e = cudaFuncSetAttribute(gemm_f8_pair_kernel<false, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairShape<SPLIT>::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2, 1, 1);
+  cfg.gridDim = dim3(2 * SPLIT, 1, 1);
   cfg.blockDim = dim3(kF8Threads, 1, 1);
-  cfg.dynamicSmemBytes = kF8Smem;
+  cfg.dynamicSmemBytes = PairShape<SPLIT>::kSmem;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.x = 2 * SPLIT; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaOccupancyMaxActiveClusters(clusters, gemm_f8_pair_kernel<true>, &cfg);
+  return cudaOccupancyMaxActiveClusters(clusters, gemm_f8_pair_kernel<true, SPLIT>, &cfg);
 }
 
-cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
+template <int SPLIT>
+cudaError_t launch(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * clusters);  // the cluster shape (2, 1, 1) is part of the kernel's declaration
+  cfg.gridDim = dim3(2 * SPLIT * clusters);  // the cluster shape is part of the kernel's declaration
   cfg.blockDim = dim3(kF8Threads);
-  cfg.dynamicSmemBytes = kF8Smem;
+  cfg.dynamicSmemBytes = PairShape<SPLIT>::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g.overlap ? 1 : 0;
-  return g.tma_store ? cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<true>, g) : cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<false>, g);
+  return g.tma_store ? cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<true, SPLIT>, g)
+                     : cudaLaunchKernelEx(&cfg, gemm_f8_pair_kernel<false, SPLIT>, g);
+}
+
+}  // namespace
+
+cudaError_t gemm_f8_pair_configure(int clusters[2]) {
+  clusters[0] = clusters[1] = 0;
+  const cudaError_t e = configure<1>(&clusters[0]);
+  return e != cudaSuccess ? e : configure<2>(&clusters[1]);
+}
+
+cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
+  return g.split == 1 ? launch<1>(g, clusters, stream) : launch<2>(g, clusters, stream);
 }
 
 }  // namespace h3b

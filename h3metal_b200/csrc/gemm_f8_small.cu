@@ -7,7 +7,7 @@
 //
 // Few rows mean that the weights are all the traffic. So the WEIGHTS take the wide side of the instruction: a tile is 128
 // rows of W (MMA M = 128, one TMEM lane and one epilogue thread per output channel) by NT rows of A (MMA N = NT, 16
-// to 128), and K is split over the CTAs of a cluster (1 to 8) until the GPU has enough copies in flight to draw the
+// to 128), and K is split over the CTAs of a cluster (2 to 8) until the GPU has enough copies in flight to draw the
 // weights at full bandwidth. The parts meet in shared memory of the cluster: CTA r adds the S partial sums of its
 // share of the rows in the order of their ranks, so that the result does not depend on who finished first.
 //
@@ -26,6 +26,8 @@ constexpr int kWRows = 128;                     // weight rows per tile = MMA M 
 constexpr int kWBytes = kWRows * kBKBytes;      // 16 KB
 constexpr int kSmallBars = 512;
 constexpr int kSmallMaxStages = 12;
+constexpr int kMaxSplit = 8;                    // CTAs of a cluster that share K
+constexpr int kPrefetchGroups = 4;
 
 template <int NT> struct Small {
   static constexpr int kStage = kWBytes + NT * kBKBytes;
@@ -71,7 +73,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = g.split;
-  const int rank = split > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+  const int rank = static_cast<int>(cluster_cta_rank());
   const int tile = blockIdx.x / split;
   const int n_blk = tile / g.m_tiles, m_blk = tile % g.m_tiles;  // tiles of the same weights are neighbours
   const int n0 = n_blk * kWRows, m0 = m_blk * NT;
@@ -89,6 +91,12 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
     for (int i = 0; i < bufs; ++i) mbar_init(acc_empty_bar(i), S::kEpiWarps);
     *cta_abort = 0;
     fence_barrier_init();
+  }
+  if (warp == 2 && lane == 0) {
+    // The weights' way from HBM into L2 may start while the kernel before still runs: 0.5 us on each of a chain of products (1 x
+    // 11520 x 3840: 10.3 -> 9.7). Eight groups gain no more than four.
+    const int ahead = min(g_end, g_begin + kPrefetchGroups);
+    for (int kb = g_begin; kb < ahead; ++kb) tma_prefetch_2d(&g.map_w, kb * kBKBytes, n0);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_holder)), S::kCols);
@@ -152,7 +160,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   } else {
     float *slots = reinterpret_cast<float *>(base_ptr + bars_off + kSmallBars) + (warp - 2) * 2 * kRows;
     const float *sw_p = g.sw + static_cast<size_t>(n_blk) * g.sw_stride;
-    // Lane t of the warp fetches the scale of its t-th row of A four groups ahead; the product with the weight block's scale
+    // Lane t of the warp fetches the scale of its t-th row of A two or four groups ahead; the product with the weight block's scale
     // goes through a slot of shared memory to all lanes. Rows past the end read another row's scale: their sums are zeros
     // (TMA fills their codes with them) and are not stored.
     const int t = part * kRows + lane;
@@ -161,7 +169,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
     for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
     // Unrolled over the fetches in flight, so that a scale stays in the register that its load wrote: moving it on would
     // wait for the load.
-    constexpr int kAhead = 4;
+    constexpr int kAhead = kRows == 16 ? 4 : 2;  // even: consecutive groups alternate between the slots
     float a_s[kAhead], w_s[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
@@ -210,38 +218,31 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   }
 
   const float bias = warp >= 2 && g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
-  if (split == 1) {
-    if (warp >= 2 && n < g.N && !*cta_abort) {
+  // every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
+  // any of them can pass the barrier below), so the ring holds the partial sums: [row of A][128]
+  float *sums = reinterpret_cast<float *>(base_ptr);
+  __syncthreads();
+  if (warp >= 2) {
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int m = m0 + part * kRows + j;
-        if (m < g.M) store_one(g, m, n, __fadd_rn(acc[j], bias));
-      }
-    }
-  } else {
-    // every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
-    // any of them can pass the barrier below), so the ring holds the partial sums: [row of A][128]
-    float *sums = reinterpret_cast<float *>(base_ptr);
-    __syncthreads();
-    if (warp >= 2) {
-#pragma unroll
-      for (int j = 0; j < kRows; ++j) sums[(part * kRows + j) * kWRows + row] = acc[j];
-    }
-    __syncwarp();
-    cluster_sync_all();
-    if (warp >= 2 && n < g.N && !*cta_abort) {
-      // this CTA finishes the rows t = rank, rank + split, ..: its epilogue warps take them in turn
-      const int rows_here = min(NT, g.M - m0);
-      for (int t = rank + split * part; t < rows_here; t += split * (S::kEpiWarps / 4)) {
-        float sum = 0.0f;
-        for (int q = 0; q < split; ++q)
-          sum = __fadd_rn(sum, ld_cluster_f32(map_to_cta(base + (t * kWRows + row) * 4, q)));
-        store_one(g, m0 + t, n, __fadd_rn(sum, bias));
-      }
-    }
-    __syncwarp();
-    cluster_sync_all();  // nobody leaves while its sums are still being read
+    for (int j = 0; j < kRows; ++j) sums[(part * kRows + j) * kWRows + row] = acc[j];
   }
+  __syncwarp();
+  cluster_sync_all();
+  if (warp >= 2 && n < g.N && !*cta_abort) {
+    // this CTA finishes the rows t = rank, rank + split, ..: its epilogue warps take them in turn
+    const int rows_here = min(NT, g.M - m0);
+    for (int t = rank + split * part; t < rows_here; t += split * (S::kEpiWarps / 4)) {
+      float part_sum[kMaxSplit], sum = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q)
+        part_sum[q] = q < split ? ld_cluster_f32(map_to_cta(base + (t * kWRows + row) * 4, q)) : 0.0f;
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q) sum = __fadd_rn(sum, part_sum[q]);
+      store_one(g, m0 + t, n, __fadd_rn(sum, bias));
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // nobody leaves while its sums are still being read
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 1) {
@@ -264,7 +265,7 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   const int groups = ((g.K + kBKBytes - 1) / kBKBytes + g.split - 1) / g.split;
   if (stages > groups) stages = groups;
   if (stages > kSmallMaxStages) stages = kSmallMaxStages;
-  const int for_sums = g.split > 1 ? (NT * kWRows * 4 + S::kStage - 1) / S::kStage : 1;  // the ring also holds the partial sums
+  const int for_sums = (NT * kWRows * 4 + S::kStage - 1) / S::kStage;  // the ring also holds the partial sums
   if (stages < for_sums) stages = for_sums;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::kThreads);
@@ -286,30 +287,35 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
 }  // namespace
 
 // Which kernel, and for few rows which tile height and how many CTAs share K. Times in nanoseconds, measured on B200 as
-// back-to-back launches (M x N x K: this kernel / CTA pairs, us): 256 x 3840 x 3840: 16.4 / 17.5; 512 x 3840 x 10240: 42.5 /
-// 38.6; 1024 x 3840 x 10240: 84.6 / 40.2; 512 x 20480 x 3840: 97.3 / 47.6. Both follow
+// back-to-back launches. All follow
 //   launch + (groups a CTA works through) * (time of a group),
-// a group taking 0.45 us on pairs and 0.475 us on 128-row tiles here.
-bool gemm_f8_choose(GemmF8Launch &g, int sms, int pair_clusters) {
+// a group taking 0.475 us on 128-row tiles here and 0.45 us on pairs; two pairs that share K pay 1.5 us to meet, and take one tile per
+// cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840 x 3840: 16.1 / 17.4 / 14.2; 512 x 3840 x 10240: 42.4 / 37.8 /
+// 26.8; 256 x 11520 x 3840: 38.8 / 18.7 / (more tiles than clusters); 512 x 20480 x 3840: 97 / 47; 128 x 3840 x 10240: 16.8 /
+// 37.0 / 25.8.
+bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]) {
   const long long groups = (g.K + kBKBytes - 1) / kBKBytes;
   const long long n_tiles = (static_cast<long long>(g.N) + kWRows - 1) / kWRows;
   g.nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   g.m_tiles = (g.M - 1) / g.nt + 1;
   const long long tiles = n_tiles * g.m_tiles;
-  // K is split while the parts still run side by side: 1 x 11520 x 3840 takes 13.0 / 11.6 / 10.3 / 13.7 us with 1 / 2 / 4 / 8
-  // parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 29.0 / 18.6 / 12.3 / 10.7 (30 tiles). Where the tiles
-  // alone fill the SMs a split only adds the exchange: 16 x 20480 x 3840 takes 16.1 / 17.7 (160 tiles).
+  // K is split two ways at least, and on while the parts still run side by side: 1 x 11520 x 3840 takes 11.6 / 10.3 / 13.7 us with
+  // 2 / 4 / 8 parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 18.6 / 12.3 / 10.7 (30 tiles).
   const int per_sm = g.nt <= 32 ? 3 : g.nt <= 64 ? 2 : 1;
   const long long slots = static_cast<long long>(sms) * per_sm;
-  g.split = 1;
+  g.split = 2;
   if (tiles < sms)
-    while (g.split < 8 && tiles * g.split * 2 <= slots && g.split * 2 <= groups) g.split *= 2;
-  if (g.nt < 128 || pair_clusters <= 0) return false;
+    while (g.split < kMaxSplit && tiles * g.split * 2 <= slots && g.split * 2 <= groups) g.split *= 2;
+  const bool can_split = groups >= 2;
+  if (can_split && g.nt < 128) return false;
   const long long waves = (tiles * g.split + slots - 1) / slots;
-  const long long here = 4500 + (g.split > 1 ? 1500 : 0) + waves * ((groups + g.split - 1) / g.split) * 475;
+  const long long here = 6000 + waves * ((groups + g.split - 1) / g.split) * 475;
   const long long pair_tiles = ((g.M - 1LL) / 256 + 1) * ((g.N - 1LL) / 256 + 1);
-  const long long pairs = 5000 + (pair_tiles + pair_clusters - 1) / pair_clusters * groups * 450;
-  return pairs < here;
+  const long long one = 5000 + (pair_tiles + pair_clusters[0] - 1) / pair_clusters[0] * groups * 450;
+  const long long two = groups >= 4 && pair_tiles <= pair_clusters[1] ? 6500 + (groups + 1) / 2 * 450 : one;
+  if (can_split && here <= one && here <= two) return false;
+  g.split = two < one ? 2 : 1;
+  return true;
 }
 
 cudaError_t gemm_f8_small_configure() {

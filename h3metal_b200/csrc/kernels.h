@@ -195,17 +195,17 @@ struct GemmF8Launch {
   long long c_stride, sa_stride, sw_stride;
   int c_dtype, M, N, K;
   int m_tiles;         // tiles of nt (pairs: 256) rows
-  int nt, split;       // few rows: rows of A per tile, CTAs that share K
+  int nt, split;       // few rows: rows of A per tile; CTAs, or pairs, that share K
   int band, tma_store; // pairs: row tiles swept per column tile; 16-bit results staged and stored by TMA
   int overlap;
   int *status;
 };
-// Fills in nt, m_tiles and split for few rows; true where CTA pairs are the faster choice.
-bool gemm_f8_choose(GemmF8Launch &g, int sms, int pair_clusters);
+// Fills in nt, m_tiles and split; true where CTA pairs are the faster choice (split: one or two pairs to a tile).
+bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]);
 cudaError_t gemm_f8_small_configure();
 cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, int sms, cudaStream_t stream);
-// CTA pairs on 256 x 256 tiles; *clusters: pairs that can be resident at once
-cudaError_t gemm_f8_pair_configure(int *clusters);
+// CTA pairs on 256 x 256 tiles; clusters: how many pairs, and how many clusters of two pairs, can be resident at once
+cudaError_t gemm_f8_pair_configure(int clusters[2]);
 cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream);
 
 }  // namespace h3b

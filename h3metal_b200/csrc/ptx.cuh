@@ -117,6 +117,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap
       : "memory");
 }
 
+// Asks for a 2-D tile to be brought into L2. Reads nothing into this CTA: memory that another kernel still writes may be asked
+// for, since L2 is where its writes go.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
+}
+
 // 3-D tile load (x innermost). Same completion mechanism as the 2-D form.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
   asm volatile(
@@ -297,6 +305,14 @@ __device__ __forceinline__ int ld_nc_s32_here(const int *p) {
 // publish no data in memory, and a cluster-scope release costs a memory fence of about 1.5 k cycles per arrival.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The two halves of a cluster barrier, for threads that need not be converged: what was written before arrive is visible to
+// whoever comes out of wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// Four values into the shared memory of a CTA of the cluster (a 16-byte aligned address from map_to_cta).
+__device__ __forceinline__ void st_cluster_v4(uint32_t dst, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 // 2-D tile load into THIS CTA's shared memory whose completion is counted on a barrier that may live in the other
 // CTA of the pair (`bar_cluster_addr` is a shared::cluster address).
