@@ -555,7 +555,8 @@ static int gemm_enqueue(h3b_ctx *ctx, const int8_t *A, int64_t a_stride, const i
   // with a short K (+3.5 % at 4096 x 3072 x 3072; -2.5 % on the 33B-class and Z-Image blocks) - and for very tall
   // products, whose output no longer fits L2 (M = 66560: +1 %).
   const bool can_stage = pair && (c_dtype == H3B_BF16 || c_dtype == H3B_F16) && gate == nullptr && ctx->pair_stages_staged >= 2 &&
-                         reinterpret_cast<uintptr_t>(C) % 16 == 0 && (c_stride * 2) % 16 == 0;
+                         reinterpret_cast<uintptr_t>(C) % 16 == 0 && (c_stride * 2) % 16 == 0 &&
+                         N % 8 == 0;  // TMA cuts a row off at whole 16-byte pieces: it would write past the last column
   const long long pair_tiles = ((M + 255LL) / 256) * ((N + 255LL) / 256);
   const bool few_tiles = pair && pair_tiles <= 3LL * ctx->pair_clusters && K <= 4096;
   const bool staged = can_stage && (ctx->store_mode == 1 || (ctx->store_mode == 0 && (few_tiles || M >= 49152)));
