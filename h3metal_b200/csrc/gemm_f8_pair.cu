@@ -3,19 +3,27 @@
 //   C[m][n] = sum_g sa[g][m] * sw[n / 128][g] * P_g[m][n] (+ bias[n]),   P_g = the group's 128 channels of A W^T
 //
 // As in gemm_f8_small.cu a group's P_g (four instructions of 32 channels, fp32 in tensor memory) is added, scaled, to
-// running sums in fp32 registers. An epilogue thread owns one row of the tile and 128 of its columns - exactly the columns
-// of one weight block, so that the scale of a group is ONE number per thread, sa * sw - and 128 running sums.
+// running sums in fp32 registers. An epilogue thread owns one row of the tile and 128 of its columns - exactly the
+// columns of one weight block, so that the scale of a group is ONE number per thread, sa * sw - and 128 running sums.
 //
-// What bounds it: the tensor cores, 512 cycles per group and SM, if the epilogue keeps up. Reading a group out of tensor
-// memory takes 256 cycles per SM and its 128 x 256 multiply-adds as many (two columns per instruction, packed fp32); two
-// accumulators of 256 columns let the MMAs of a group run while the group before is read.
+// What bounds it: a group's MMAs take 512 cycles; reading it out of tensor memory, 128 x 256 values per SM, and the
+// multiply-adds (two columns per packed instruction) take about 250 each, beside the MMAs of the next group, for
+// which there is a second accumulator of 256 columns. An accumulator goes round through the pair (MMAs done -> both
+// epilogues -> leader), and two messages between SMs cost 0.6 us, so a group takes 860 cycles. Measured, back to back
+// for a second under the board's power cap: 17408 x 18432 x 6144 in 1.87 ms = 2.10 PFLOP/s at 1.46 GHz, 9.7 of 16.4
+// kflop per clock and SM (60 %); three launches from idle 2.39 PFLOP/s. With an epilogue that only hands accumulators
+// back: 2.24; without its multiply-adds: 2.27. Not taken: three accumulators of 160 columns (2.48 against 1.96 ms:
+// more bytes per multiply, and the issuing thread's four instructions and commit per group no longer hide), MMAs of
+// 128 columns into four accumulators (+17 %: A is read twice from shared memory), single CTAs on 128 x 256 tiles (+10
+// %, half as many more bytes), sixteen epilogue warps (+10 %).
 //
-// Roles per CTA (rank 0 = leader): warp 0 TMA producer (own 128 rows of A, own half of the 256 rows of W per group, bytes
-// of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3 idle, warps 4..11
-// epilogue: four lane quarters x two halves of 128 columns; the first four warps hand them most of their registers. 16-bit
-// results are staged in shared memory as 128-byte-swizzled panels and stored by TMA while the next tile runs; fp32 results
-// and unaligned outputs are turned there and stored row by row. Set-up overlaps the kernel before (programmatic stream
-// serialization). All waits are bounded. No load uses multicast.
+// Roles per CTA (rank 0 of a pair = leader): warp 0 TMA producer (own 128 rows of A, own half of the 256 rows of W
+// per group, bytes of both CTAs counted on the leader's barrier), warp 1 of the leader issues the MMAs, warps 2 and 3
+// idle, warps 4..11 epilogue: four lane quarters x two halves of 128 columns; the first four warps hand them most of
+// their registers. One commit per group says both that the stage may be refilled and that the accumulator may be
+// read. 16-bit results are staged in shared memory as 128-byte-swizzled panels and stored by TMA while the next tile
+// runs; fp32 results and unaligned outputs are turned there and stored row by row. Set-up overlaps the kernel before
+// (programmatic stream serialization). All waits are bounded. No load uses multicast.
 #include <cuda.h>
 
 #include "gemm_common.cuh"
@@ -36,8 +44,8 @@ constexpr int kF8RegsIssue = 104, kF8RegsEpi = 200;
 constexpr int kF8OutWarp = 2 * kOutPanel;           // a warp's 32 rows x 128 two-byte columns
 constexpr int kF8MailWarp = 32 * 128 * 4;           // a warp's 32 x 128 fp32 sums
 
-// SPLIT 1: a pair has the whole of K, eight warps stage results. SPLIT 2: two pairs of a cluster have half of K each for ONE tile
-// per cluster; four warps of each stage results and receive the other pair's sums.
+// SPLIT 1: a pair has the whole of K, eight warps stage results. SPLIT 2: two pairs of a cluster have half of K each
+// for ONE tile per cluster; four warps of each stage results and receive the other pair's sums.
 template <int SPLIT> struct PairShape {
   static constexpr int kStages = SPLIT == 1 ? 5 : 4;
   static constexpr int kMailOff = kStages * kF8Stage;
@@ -53,6 +61,7 @@ __device__ __forceinline__ void scale_add16(const uint32_t (&p)[16], float2 s2, 
   for (int j = 0; j < 8; ++j)
     acc[j] = __ffma2_rn(make_float2(__uint_as_float(p[2 * j]), __uint_as_float(p[2 * j + 1])), s2, acc[j]);
 }
+
 // 32 columns of a warp's 32 rows, from (m, n) on, without TMA: turned in 4 KB of shared memory (piece p of row r sits at
 // p ^ (r & 7)) so that a store instruction writes whole rows. A thread's own row, stored as it lies in registers, would
 // touch 32 lines per instruction: 575 against 204 us at 4608 x 11520 x 3840.
@@ -68,7 +77,8 @@ __device__ __forceinline__ void store_chunk(const GemmF8Launch &g, float *buf, i
     for (int i = 0; i < 8; ++i) {  // four rows per instruction
       const int r = 4 * i + (lane >> 3);
       const float4 x = reinterpret_cast<const float4 *>(buf)[r * 8 + (q ^ (r & 7))];
-      if (m + r < g.M) *reinterpret_cast<float4 *>(static_cast<float *>(g.c) + static_cast<size_t>(m + r) * g.c_stride + n + 4 * q) = x;
+      float *dst = static_cast<float *>(g.c) + static_cast<size_t>(m + r) * g.c_stride + n + 4 * q;
+      if (m + r < g.M) *reinterpret_cast<float4 *>(dst) = x;
     }
   } else if (n + lane < g.N) {
     const int rows = min(32, g.M - m);
@@ -192,7 +202,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
             const uint32_t d = tmem_base + buf.s * kF8BN;
 #pragma unroll
             for (int k = 0; k < kBKBytes / 32; ++k) umma_f8_pair(d, ad + 2u * k, bd + 2u * k, idesc, k ? 1u : 0u);
-            umma_commit_pair(done_bar(s), static_cast<uint16_t>(3u << leader_cta));  // the stage may be refilled, the accumulator read
+            umma_commit_pair(done_bar(s), static_cast<uint16_t>(3u << leader_cta));
             pos.advance(stages);
             buf.advance(2);
           }
@@ -217,7 +227,8 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
       const TileCoord tc = tile_coord(tile, g.m_tiles, n_tiles, g.band);
       const int m0 = tc.m_blk * 256 + static_cast<int>(rank) * 128, n0 = tc.n_blk * kF8BN + part * kF8Cols;
       const int m = m0 + row;
-      // rows and columns past the end compute zeros (TMA fills their codes with them) and are not stored: any scale will do
+      // rows and columns past the end compute zeros (TMA fills their codes with them) and are not stored: any scale
+      // will do
       const int m_s = min(m, g.M - 1), n_s = min(n0 / 128, n_blocks - 1);
       float2 acc[kF8Cols / 2];
 #pragma unroll
@@ -256,9 +267,10 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
         buf ^= 1u;
       }
       if constexpr (SPLIT > 1) {
-        // Each pair finishes one column half: the warps of the other half leave their sums with the same warp quarter of the
-        // other pair's CTA with the same rows, 16 bytes per lane at [piece of four columns][lane]. A cluster has one tile, so
-        // the two barriers of the cluster, here and at the end, are all it takes; a warp that gave up meets them too.
+        // Each pair finishes one column half: the warps of the other half leave their sums with the same warp quarter
+        // of the other pair's CTA with the same rows, 16 bytes per lane at [piece of four columns][lane]. A cluster
+        // has one tile, so the two barriers of the cluster, here and at the end, are all it takes; a warp that gave
+        // up meets them too.
         if (ok && part != pair) {
           const uint32_t dst = map_to_cta(base + P::kMailOff + quarter * kF8MailWarp + lane * 16, cta ^ 2u);
 #pragma unroll
@@ -340,9 +352,10 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
 
 template <int SPLIT>
 cudaError_t configure(int *clusters) {
-  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel<true, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairShape<SPLIT>::kSmem);
+  constexpr int smem = static_cast<int>(PairShape<SPLIT>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(gemm_f8_pair_kernel<true, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(gemm_f8_pair_kernel<false, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairShape<SPLIT>::kSmem);
+  e = cudaFuncSetAttribute(gemm_f8_pair_kernel<false, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * SPLIT, 1, 1);

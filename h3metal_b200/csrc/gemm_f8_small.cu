@@ -2,17 +2,23 @@
 // P_g[m][n] = sum over the 128 channels of group g of A[m][k] * W[n][k].
 //
 // The tensor core multiplies codes and accumulates a group in fp32; the scales differ from group to group, so every
-// group's P_g leaves tensor memory on its own and is added, scaled, to running sums that stay in fp32 registers:
-// one fused multiply-add per output and group, no rounding to fewer bits before the end.
+// group's P_g leaves tensor memory on its own and is added, scaled, to running sums that stay in fp32 registers: one
+// fused multiply-add per output and group, no rounding to fewer bits before the end.
 //
-// Few rows mean that the weights are all the traffic. So the WEIGHTS take the wide side of the instruction: a tile is 128
-// rows of W (MMA M = 128, one TMEM lane and one epilogue thread per output channel) by NT rows of A (MMA N = NT, 16
-// to 128), and K is split over the CTAs of a cluster (2 to 8) until the GPU has enough copies in flight to draw the
-// weights at full bandwidth. The parts meet in shared memory of the cluster: CTA r adds the S partial sums of its
+// Few rows mean that the weights are all the traffic. So the WEIGHTS take the wide side of the instruction: a tile is
+// 128 rows of W (MMA M = 128, one TMEM lane and one epilogue thread per output channel) by NT rows of A (MMA N = NT,
+// 16 to 128), and K is split over the CTAs of a cluster (2 to 8) until the GPU has enough copies in flight to draw
+// the weights at full bandwidth. The parts meet in shared memory of the cluster: CTA r adds the S partial sums of its
 // share of the rows in the order of their ranks, so that the result does not depend on who finished first.
 //
-// Roles: warp 0 TMA producer (W tile 16 KB and NT x 128 bytes of A per group), warp 1 MMA issuer, warps 2..5 epilogue.
-// Out-of-range rows and channels are zero-filled by TMA. All waits are bounded. No load uses multicast.
+// Roles: warp 0 TMA producer (W tile 16 KB and NT x 128 bytes of A per group), warp 1 MMA issuer, warps 2.. epilogue,
+// four lane quarters x parts of up to 32 rows of A. Out-of-range rows and channels are zero-filled by TMA. All waits
+// are bounded. No load uses multicast.
+//
+// What bounds it: HBM for few rows. 1 x 11520 x 3840, one of a chain of launches: 9.8 us = 4.5 TB/s; the weights
+// themselves stream at 6.2 TB/s for 7.1 us of them, the rest is the first tile's latency (1.3 us), the two cluster
+// barriers and the exit. For 64 and more rows the one issuing thread: two barrier polls, four instructions and a
+// commit take 600 to 850 cycles per group.
 #include <cuda.h>
 
 #include "gemm_common.cuh"
@@ -93,8 +99,8 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
     fence_barrier_init();
   }
   if (warp == 2 && lane == 0) {
-    // The weights' way from HBM into L2 may start while the kernel before still runs: 0.5 us on each of a chain of products (1 x
-    // 11520 x 3840: 10.3 -> 9.7). Eight groups gain no more than four.
+    // The weights' way from HBM into L2 may start while the kernel before still runs: 0.5 us on each of a chain of
+    // products (1 x 11520 x 3840: 10.3 -> 9.7). Eight groups gain no more than four.
     const int ahead = min(g_end, g_begin + kPrefetchGroups);
     for (int kb = g_begin; kb < ahead; ++kb) tma_prefetch_2d(&g.map_w, kb * kBKBytes, n0);
   }
@@ -160,9 +166,9 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   } else {
     float *slots = reinterpret_cast<float *>(base_ptr + bars_off + kSmallBars) + (warp - 2) * 2 * kRows;
     const float *sw_p = g.sw + static_cast<size_t>(n_blk) * g.sw_stride;
-    // Lane t of the warp fetches the scale of its t-th row of A two or four groups ahead; the product with the weight block's scale
-    // goes through a slot of shared memory to all lanes. Rows past the end read another row's scale: their sums are zeros
-    // (TMA fills their codes with them) and are not stored.
+    // Lane t of the warp fetches the scale of its t-th row of A two or four groups ahead; the product with the weight
+    // block's scale goes through a slot of shared memory to all lanes. Rows past the end read another row's scale:
+    // their sums are zeros (TMA fills their codes with them) and are not stored.
     const int t = part * kRows + lane;
     const float *sa_p = g.sa + (lane < kRows && m0 + t < g.M ? m0 + t : m0);
 #pragma unroll
@@ -269,7 +275,10 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   if (stages < for_sums) stages = for_sums;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = fixed + static_cast<size_t>(stages) * S::kStage;
+  // Never more CTAs on an SM than its 512 columns of tensor memory serve: a CTA that waits for columns while its cluster waits for it
+  // could otherwise close a circle with another cluster.
+  const size_t needed = fixed + static_cast<size_t>(stages) * S::kStage, least = 233472 / (512 / S::kCols + 1);
+  cfg.dynamicSmemBytes = needed > least ? needed : least;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -278,29 +287,29 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g.overlap ? 2 : 1;
-  // A stage's barrier tells its uses apart by their parity alone. The epilogue, which waits on it too, must therefore be less
-  // than a whole ring behind the MMAs, and it can be as many groups behind as there are accumulators.
+  // A stage's barrier tells its uses apart by their parity alone. The epilogue, which waits on it too, must therefore
+  // be less than a whole ring behind the MMAs, and it can be as many groups behind as there are accumulators.
   const int bufs = stages < S::kBufs ? stages : S::kBufs;
   return cudaLaunchKernelEx(&cfg, gemm_f8_small_kernel<NT>, g, stages, bufs);
 }
 
 }  // namespace
 
-// Which kernel, and for few rows which tile height and how many CTAs share K. Times in nanoseconds, measured on B200 as
-// back-to-back launches. All follow
+// Which kernel, and for few rows which tile height and how many CTAs share K. Times in nanoseconds, measured on B200
+// as back-to-back launches. All follow
 //   launch + (groups a CTA works through) * (time of a group),
-// a group taking 0.475 us on 128-row tiles here and 0.45 us on pairs; two pairs that share K pay 1.5 us to meet, and take one tile per
-// cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840 x 3840: 16.1 / 17.4 / 14.2; 512 x 3840 x 10240: 42.4 / 37.8 /
-// 26.8; 256 x 11520 x 3840: 38.8 / 18.7 / (more tiles than clusters); 512 x 20480 x 3840: 97 / 47; 128 x 3840 x 10240: 16.8 /
-// 37.0 / 25.8.
+// a group taking 0.475 us on 128-row tiles here and 0.45 us on pairs; two pairs that share K pay 1.5 us to meet, and
+// take one tile per cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840 x 3840: 16.1 / 17.4 / 14.2; 512 x
+// 3840 x 10240: 42.4 / 37.8 / 26.8; 256 x 11520 x 3840: 38.8 / 18.7 / (more tiles than clusters); 512 x 20480 x 3840:
+// 97 / 47; 128 x 3840 x 10240: 16.8 / 37.0 / 25.8.
 bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]) {
   const long long groups = (g.K + kBKBytes - 1) / kBKBytes;
   const long long n_tiles = (static_cast<long long>(g.N) + kWRows - 1) / kWRows;
   g.nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   g.m_tiles = (g.M - 1) / g.nt + 1;
   const long long tiles = n_tiles * g.m_tiles;
-  // K is split two ways at least, and on while the parts still run side by side: 1 x 11520 x 3840 takes 11.6 / 10.3 / 13.7 us with
-  // 2 / 4 / 8 parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 18.6 / 12.3 / 10.7 (30 tiles).
+  // K is split two ways at least, and on while the parts still run side by side: 1 x 11520 x 3840 takes 11.6 / 10.3 /
+  // 13.7 us with 2 / 4 / 8 parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 18.6 / 12.3 / 10.7 (30 tiles).
   const int per_sm = g.nt <= 32 ? 3 : g.nt <= 64 ? 2 : 1;
   const long long slots = static_cast<long long>(sms) * per_sm;
   g.split = 2;
