@@ -275,8 +275,8 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   if (stages < for_sums) stages = for_sums;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::kThreads);
-  // Never more CTAs on an SM than its 512 columns of tensor memory serve: a CTA that waits for columns while its cluster waits for it
-  // could otherwise close a circle with another cluster.
+  // Never more CTAs on an SM than its 512 columns of tensor memory serve: a CTA that waits for columns while its
+  // cluster waits for it could otherwise close a circle with another cluster.
   const size_t needed = fixed + static_cast<size_t>(stages) * S::kStage, least = 233472 / (512 / S::kCols + 1);
   cfg.dynamicSmemBytes = needed > least ? needed : least;
   cfg.stream = stream;

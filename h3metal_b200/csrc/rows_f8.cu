@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) quant_f8_kernel(const QuantArgs p) {
   encode_piece(v, n, p.out + m * p.out_stride + piece * kPiece, p.sa + group * p.sa_stride + m, n > 0 && (piece & 7) == 0);
 }
 
-// ---- norm: a CTA has a row at a time, C pieces per thread --------------------------------------------------------------------
+// ---- norm: a CTA has a row at a time, C pieces per thread ---------------------------------------------------------
 struct RmsArgs {
   const void *x, *y, *w;
   void *res;
@@ -261,7 +261,8 @@ __global__ void __maxnreg__(WARPS == 32 ? 64 : C == 1 ? 80 : 128) rms_f8_kernel(
     fetch(m, 0);
     gain_of(0, gain);
   }
-  for (int turn = 0; m < p.M; m += step, turn ^= 1) {  // the same for all threads of a row, and rows only meet a barrier alone
+  // the same trips for all threads of a row; only rows that are alone in their CTA meet a barrier
+  for (int turn = 0; m < p.M; m += step, turn ^= 1) {
     float2 v[C][kPiece / 2];
     float2 ss2 = both(0.0f);
 #pragma unroll

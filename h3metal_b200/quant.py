@@ -94,15 +94,26 @@ def _e4m3_values() -> np.ndarray:
     return np.where(exp == 0, man * 2.0 ** -9, (8 + man) * 2.0 ** (exp - 10.0))
 
 
+@functools.lru_cache(maxsize=1)
+def _e4m3_codes() -> np.ndarray:
+    """The code of k * 2^-9 for every k that is an e4m3 value (the smallest subnormal is 2^-9), by k."""
+    table = np.zeros(int(F8_TOP * 512) + 1, np.uint8)
+    table[(_e4m3_values() * 512).astype(np.int64)] = np.arange(127, dtype=np.uint8)
+    return table
+
+
 def e4m3_bits(a: np.ndarray) -> np.ndarray:
     """Values -> e4m3 codes (uint8), round to nearest even, saturating at +-448; NaN -> 0x7F."""
-    a = np.asarray(a, dtype=np.float64)
-    grid = _e4m3_values()
-    mag = np.minimum(np.where(np.isnan(a), 0.0, np.abs(a)), F8_TOP)
-    hi = np.clip(np.searchsorted(grid, mag), 1, 126)
-    below, above = mag - grid[hi - 1], grid[hi] - mag
-    code = np.where((above < below) | ((above == below) & (hi % 2 == 0)), hi, hi - 1).astype(np.uint8)
-    return np.where(np.isnan(a), np.uint8(0x7F), code | (np.signbit(a).astype(np.uint8) << 7)).astype(np.uint8)
+    a = np.asarray(a)
+    if a.dtype not in (np.float32, np.float64):
+        a = a.astype(np.float64)
+    nan = np.isnan(a)
+    mag = np.minimum(np.where(nan, a.dtype.type(0), np.abs(a)), a.dtype.type(F8_TOP))
+    _, exp = np.frexp(mag)                     # mag = [0.5, 1) * 2^exp: eight steps per power of two, from 2^-6 on
+    shift = 4 - np.maximum(exp, -5)
+    steps = np.rint(np.ldexp(mag, shift))      # exact: a power of two apart; rint goes to even
+    code = _e4m3_codes()[np.ldexp(steps, 9 - shift).astype(np.int64)]
+    return np.where(nan, np.uint8(0x7F), code | (np.signbit(a).astype(np.uint8) << 7)).astype(np.uint8)
 
 
 def e4m3_to_f32(u: np.ndarray) -> np.ndarray:
