@@ -86,7 +86,7 @@ struct h3b_ctx {
   int overlap = 1;  // programmatic dependent launch of the path's main kernels (h3b_set_launch_overlap); on by default
   int pair_stages = 0, pair_clusters = 0;  // CTA-pair product: ring depth and resident clusters (0 = unavailable)
   int pair_stages_staged = 0;              // ring depth when 64 KB of shared memory stage the outputs for TMA stores
-  int f8_pair_clusters[2] = {0, 0};        // the same for the block-scaled product: pairs, clusters of two pairs
+  h3b::F8Clusters f8_resident;             // the same for the block-scaled product's kernels
   int store_mode = 0;                      // staged (TMA) stores of the pair product: 0 automatic, 1 whenever possible, -1 never
   uint64_t launches = 0;
   std::string name;
@@ -276,8 +276,8 @@ h3b_ctx *h3b_open(int device) {
   ctx->encode = reinterpret_cast<EncodeTiledFn>(fn);
   if ((e = h3b::gemm_configure(device)) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
   if ((e = h3b::gemm_pair_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
-  if ((e = h3b::gemm_f8_small_configure()) != cudaSuccess) return bail("cudaFuncSetAttribute(max dynamic shared memory)", e);
-  if ((e = h3b::gemm_f8_pair_configure(ctx->f8_pair_clusters)) != cudaSuccess) return bail("gemm_f8 set-up", e);
+  if ((e = h3b::gemm_f8_small_configure(ctx->f8_resident.rows128)) != cudaSuccess) return bail("gemm_f8 set-up", e);
+  if ((e = h3b::gemm_f8_pair_configure(&ctx->f8_resident.pairs, &ctx->f8_resident.twos)) != cudaSuccess) return bail("gemm_f8 set-up", e);
   ctx->pair_stages = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, false);
   ctx->pair_stages_staged = h3b::gemm_pair_pick_stages(ctx->prop.sharedMemPerBlockOptin, true);
   ctx->pair_clusters = ctx->pair_stages >= 2 ? h3b::gemm_pair_max_clusters(ctx->pair_stages) : 0;
@@ -907,8 +907,8 @@ int h3b_gemm_f8(h3b_ctx *ctx, const h3b_gemm_f8_args *args) {
   g.c_dtype = c_dtype; g.M = M; g.N = N; g.K = K;
   g.overlap = (ctx->overlap != 0 && !ctx->profile) ? 1 : 0;
   g.status = ctx->status_dev;
-  if (ctx->f8_pair_clusters[0] < 1) return fail("gemm_f8: the device holds no CTA pair of this kernel");
-  const bool pair = h3b::gemm_f8_choose(g, ctx->prop.multiProcessorCount, ctx->f8_pair_clusters);
+  if (ctx->f8_resident.pairs < 1) return fail("gemm_f8: the device holds no CTA pair of this kernel");
+  const bool pair = h3b::gemm_f8_choose(g, ctx->prop.multiProcessorCount, ctx->f8_resident);
   const CUtensorMap *m;
   if (pair) {
     g.m_tiles = (M - 1) / 256 + 1;
@@ -932,7 +932,8 @@ int h3b_gemm_f8(h3b_ctx *ctx, const h3b_gemm_f8_args *args) {
     }
     cudaEvent_t ps = nullptr;
     if (ctx->before_launch(&ps)) return -1;
-    const int resident = ctx->f8_pair_clusters[g.split - 1], clusters = static_cast<int>(tiles < resident ? tiles : resident);
+    const int resident = g.split == 1 ? ctx->f8_resident.pairs : ctx->f8_resident.twos;
+    const int clusters = static_cast<int>(tiles < resident ? tiles : resident);
     return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_pair(g, clusters, ctx->stream));
   }
   if (((N - 1LL) / 128 + 1) * g.m_tiles * g.split > 0x7FFFFFFFLL) return fail("gemm_f8: too many tiles for one launch");

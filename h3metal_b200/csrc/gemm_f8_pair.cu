@@ -387,10 +387,10 @@ cudaError_t launch(const GemmF8Launch &g, int clusters, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t gemm_f8_pair_configure(int clusters[2]) {
-  clusters[0] = clusters[1] = 0;
-  const cudaError_t e = configure<1>(&clusters[0]);
-  return e != cudaSuccess ? e : configure<2>(&clusters[1]);
+cudaError_t gemm_f8_pair_configure(int *pairs, int *twos) {
+  *pairs = *twos = 0;
+  const cudaError_t e = configure<1>(pairs);
+  return e != cudaSuccess ? e : configure<2>(twos);
 }
 
 cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream) {

@@ -264,7 +264,9 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>((g.N + kWRows - 1) / kWRows) * g.m_tiles * g.split;
   // Ring depth: what is left of an SM's 228 KB for each of the CTAs that share it, and no more than there are groups.
   const int want = static_cast<int>((grid + sms - 1) / sms);
-  const int per_sm = want < S::kPerSm ? want : S::kPerSm;
+  // Room for a second CTA even where one per SM would do: a cluster lies inside a GPC, and clusters of eight CTAs that
+  // take a whole SM each do not pack (24 x 2048 x 8192 in 8 parts, 128 CTAs: 13.5 us, with room for two CTAs to an SM 7.7).
+  const int per_sm = want >= S::kPerSm ? S::kPerSm : want < 2 && S::kPerSm > 1 ? 2 : want;
   const int fixed = 1024 + kSmallBars + S::kScaleBytes;
   const int room = 233472 / per_sm - 1024;  // the runtime keeps 1 KB per CTA
   int stages = (room - fixed) / S::kStage;
@@ -298,11 +300,12 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
 // Which kernel, and for few rows which tile height and how many CTAs share K. Times in nanoseconds, measured on B200
 // as back-to-back launches. All follow
 //   launch + (groups a CTA works through) * (time of a group),
-// a group taking 0.475 us on 128-row tiles here and 0.45 us on pairs; two pairs that share K pay 1.5 us to meet, and
-// take one tile per cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840 x 3840: 16.1 / 17.4 / 14.2; 512 x
-// 3840 x 10240: 42.4 / 37.8 / 26.8; 256 x 11520 x 3840: 38.8 / 18.7 / (more tiles than clusters); 512 x 20480 x 3840:
-// 97 / 47; 128 x 3840 x 10240: 16.8 / 37.0 / 25.8.
-bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]) {
+// a group taking 0.5 us on 128-row tiles here, where every wave of CTAs starts anew, and 0.45 us on pairs; two pairs
+// that share K pay 1.5 us to meet, and take one tile per cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840
+// x 3840: 15.2 / 17.4 / 13.8; 512 x 3840 x 10240: 42.4 / 37.8 / 26.8; 128 x 3840 x 3840: 10.4 / 17 / 13.6; 128 x 20480
+// x 3840: 44.6 / 33.2; 512 x 20480 x 3840: 97 / 47. Over nine M of 1 to 640 and seven N x K the choice is within 2 % of
+// the best.
+bool gemm_f8_choose(GemmF8Launch &g, int sms, const F8Clusters &resident) {
   const long long groups = (g.K + kBKBytes - 1) / kBKBytes;
   const long long n_tiles = (static_cast<long long>(g.N) + kWRows - 1) / kWRows;
   g.nt = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
@@ -310,30 +313,48 @@ bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]) {
   const long long tiles = n_tiles * g.m_tiles;
   // K is split two ways at least, and on while the parts still run side by side: 1 x 11520 x 3840 takes 11.6 / 10.3 /
   // 13.7 us with 2 / 4 / 8 parts (90 tiles, three CTAs to an SM), 16 x 3840 x 10240 18.6 / 12.3 / 10.7 (30 tiles).
+  // 128-row tiles have an SM each, and what fits is a matter of whole clusters.
   const int per_sm = g.nt <= 32 ? 3 : g.nt <= 64 ? 2 : 1;
-  const long long slots = static_cast<long long>(sms) * per_sm;
   g.split = 2;
-  if (tiles < sms)
-    while (g.split < kMaxSplit && tiles * g.split * 2 <= slots && g.split * 2 <= groups) g.split *= 2;
-  const bool can_split = groups >= 2;
+  int room = 0;  // clusters of g.split that run side by side
+  for (int i = 0; i < 3; ++i) {
+    const int split = 2 << i;
+    const int fits = per_sm == 1 ? resident.rows128[i] : sms * per_sm / split;
+    if (i > 0 && (tiles >= sms || tiles > fits || split > groups)) break;
+    g.split = split;
+    room = fits;
+  }
+  const bool can_split = groups >= 2 && room > 0;
   if (can_split && g.nt < 128) return false;
-  const long long waves = (tiles * g.split + slots - 1) / slots;
-  const long long here = 6000 + waves * ((groups + g.split - 1) / g.split) * 475;
+  const long long waves = room > 0 ? (tiles + room - 1) / room : 0;
+  const long long here = 2000 + waves * (4500 + (groups + g.split - 1) / g.split * 500);
   const long long pair_tiles = ((g.M - 1LL) / 256 + 1) * ((g.N - 1LL) / 256 + 1);
-  const long long one = 5000 + (pair_tiles + pair_clusters[0] - 1) / pair_clusters[0] * groups * 450;
-  const long long two = groups >= 4 && pair_tiles <= pair_clusters[1] ? 6500 + (groups + 1) / 2 * 450 : one;
+  const long long one = 5000 + (pair_tiles + resident.pairs - 1) / resident.pairs * groups * 450;
+  const long long two = groups >= 4 && pair_tiles <= resident.twos ? 6500 + (groups + 1) / 2 * 450 : one;
   if (can_split && here <= one && here <= two) return false;
   g.split = two < one ? 2 : 1;
   return true;
 }
 
-cudaError_t gemm_f8_small_configure() {
+cudaError_t gemm_f8_small_configure(int rows128[3]) {
   cudaError_t e;
-#define H3B_F8_CFG(NT)                                                                                                   \
-  if ((e = cudaFuncSetAttribute(gemm_f8_small_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448)) != cudaSuccess) \
-    return e;
+#define H3B_F8_CFG(NT)                                                                                               \
+  e = cudaFuncSetAttribute(gemm_f8_small_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);           \
+  if (e != cudaSuccess) return e;
   H3B_F8_CFG(16) H3B_F8_CFG(32) H3B_F8_CFG(64) H3B_F8_CFG(128)
 #undef H3B_F8_CFG
+  for (int i = 0; i < 3; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 << i);
+    cfg.blockDim = dim3(Small<128>::kThreads);
+    cfg.dynamicSmemBytes = 232448;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2 << i; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaOccupancyMaxActiveClusters(&rows128[i], gemm_f8_small_kernel<128>, &cfg)) != cudaSuccess) return e;
+  }
   return cudaSuccess;
 }
 

@@ -200,12 +200,17 @@ struct GemmF8Launch {
   int overlap;
   int *status;
 };
+// How many clusters of each kind a device holds at once.
+struct F8Clusters {
+  int pairs = 0, twos = 0;         // CTA pairs; clusters of two pairs
+  int rows128[3] = {0, 0, 0};      // few-row kernel with 128-row tiles: clusters of 2, 4 and 8 CTAs
+};
 // Fills in nt, m_tiles and split; true where CTA pairs are the faster choice (split: one or two pairs to a tile).
-bool gemm_f8_choose(GemmF8Launch &g, int sms, const int pair_clusters[2]);
-cudaError_t gemm_f8_small_configure();
+bool gemm_f8_choose(GemmF8Launch &g, int sms, const F8Clusters &resident);
+cudaError_t gemm_f8_small_configure(int rows128[3]);
 cudaError_t launch_gemm_f8_small(const GemmF8Launch &g, int sms, cudaStream_t stream);
-// CTA pairs on 256 x 256 tiles; clusters: how many pairs, and how many clusters of two pairs, can be resident at once
-cudaError_t gemm_f8_pair_configure(int clusters[2]);
+// CTA pairs on 256 x 256 tiles
+cudaError_t gemm_f8_pair_configure(int *pairs, int *twos);
 cudaError_t launch_gemm_f8_pair(const GemmF8Launch &g, int clusters, cudaStream_t stream);
 
 }  // namespace h3b

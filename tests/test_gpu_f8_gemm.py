@@ -62,7 +62,7 @@ def run(gpu, a, sa, w, sw, M, N, K, dtype, bias=None, c_stride=None, sa_stride=N
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 300, 1000), (2, 129, 127), (5, 64, 3840), (16, 256, 129), (17, 130, 2048), (32, 384, 640),
          (33, 1000, 400), (64, 512, 1024), (65, 257, 777), (100, 771, 1000), (128, 128, 16384), (129, 640, 256), (255, 256, 128),
          (256, 256, 384), (257, 513, 1040), (300, 1280, 512), (700, 700, 300), (1024, 512, 256), (1100, 2304, 640),
-         (2600, 2304, 300), (20, 11400, 3840), (64, 9000, 640), (7, 20000, 384)]
+         (2600, 2304, 300), (20, 11400, 3840), (64, 9000, 640), (7, 20000, 384), (24, 2048, 8192), (160, 1024, 2048)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
