@@ -146,6 +146,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
       const uint64_t wd0 = umma_smem_desc(base, 1024, 2);
       const uint64_t ad0 = umma_smem_desc(base + kWBytes, 1024, 2);
       RingPos pos, buf;
+      bool issued = false;
       for (int kb = g_begin; kb < g_end; ++kb) {
         const uint32_t s = pos.s;
         // two polls in flight at once: a barrier's answer takes about 80 cycles, a third of the instructions' own issue
@@ -161,6 +162,12 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
         umma_commit(done_bar(s));
         pos.advance(stages);
         buf.advance(bufs);
+        issued = true;
+      }
+      if (*cta_abort && issued) {  // instructions still in flight must finish before tensor memory is given up
+        pos.retreat(stages);
+        int dummy_abort = 0;
+        mbar_wait(done_bar(pos.s), pos.ph, &dummy_abort, g.status, kStatusDrainTimeout, kDrainLimitCycles);
       }
     }
   } else {
@@ -224,10 +231,16 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   }
 
   const float bias = warp >= 2 && g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
-  // every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
-  // any of them can pass the barrier below), so the ring holds the partial sums: [row of A][128]
+  // Every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
+  // any of them can pass the barrier below), so tensor memory can go and the ring holds the partial sums: [row of
+  // A][128]
   float *sums = reinterpret_cast<float *>(base_ptr);
+  tc_fence_before_sync();
   __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, S::kCols);
+  }
   if (warp >= 2) {
 #pragma unroll
     for (int j = 0; j < kRows; ++j) sums[(part * kRows + j) * kWRows + row] = acc[j];
@@ -249,12 +262,6 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   }
   __syncwarp();
   cluster_sync_all();  // nobody leaves while its sums are still being read
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem_base, S::kCols);
-  }
 }
 
 template <int NT>
