@@ -2,12 +2,12 @@
 //
 //   rms_f8     h = x (+ y), rounded to x's type and kept;  v = h * rsqrt(mean(h^2) + eps) * w
 //   quant_f8   v = x,  or  v = x[:, :D] * silu(x[:, D:2D])
-//   both       s[g][m] = max(amax over the group |v| / 448, 2^-126), 1 where the group is all zero;  code = e4m3(v / s)
+//   both       s[g][m] = max(amax over the group |v| / 448, 2^-126), 1 where the group is all zero;  code = e4m3(v * (1 / s))
 //
 // 448 is the largest finite e4m3 value. The floor 2^-126 keeps 1 / s finite: groups whose largest magnitude is below
 // 448 * 2^-126 lose their smallest codes instead of turning into 0 * inf. Codes are the nearest e4m3 value (ties to
-// even) of v * (1 / s); the reciprocal is one rounding away from a division, which matters only to values within
-// 2^-23 of the middle between two codes. A NaN keeps its own place (code 0x7F) and the group's scale comes from the
+// even) of v * (1 / s): two roundings of 2^-24 each away from v / s, which matters only to values within 2^-23 of the
+// middle between two codes - to which both codes are equally near. A NaN keeps its own place (code 0x7F) and the group's scale comes from the
 // other values; an infinity makes the scale infinite, and the group NaN when it is read back. Sums, statistics and
 // scales are fp32. The stream h is rounded to x's type BEFORE it is normed, as if the addition had been a call of its
 // own: what is normed is what the next layer adds to.

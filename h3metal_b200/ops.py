@@ -296,7 +296,8 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
            out_stride: int | None = None, sa_stride: int | None = None):
     """out, sa = e4m3 codes and scales of rmsnorm(x) * w (w [D], no offset). With y, first x + y, rounded to x's type and
     kept in res (x itself by default), is what is normed. x, y and w are bf16, f16 or f32, each its own. out: "f8" rows of
-    quant.f8_stride(D) bytes; sa: fp32 [ceil(D / 128)][M], a group's scales of all rows side by side."""
+    quant.f8_stride(D) bytes; sa: fp32 [ceil(D / 128)][M], a group's scales of all rows side by side. A code is
+    e4m3(v * (1 / scale)) in fp32 steps (quant.f8_codes)."""
     if M <= 0 or D <= 0:
         raise ValueError("rms_f8: M and D must be positive")
     x_stride, out_stride, sa_stride = x_stride or D, out_stride or f8_stride(D), sa_stride or M

@@ -128,9 +128,18 @@ def f8_stride(k: int) -> int:
     return -(-k // 16) * 16
 
 
+def f8_codes(v: np.ndarray, s: np.ndarray) -> np.ndarray:
+    """The codes that rms_f8 and quant_f8 (ops) write for fp32 values v under scales s (broadcast): e4m3(v * (1 / s)), each
+    step one fp32 rounding. The nearest code to v / s, or either neighbour where v / s lies within 2^-23 of itself of the
+    middle between two codes."""
+    with np.errstate(over="ignore", invalid="ignore"):
+        return e4m3_bits(v.astype(np.float32, copy=False) * (np.float32(1) / s.astype(np.float32, copy=False)))
+
+
 def quant_f8(w: np.ndarray):
     """Weight [N][K] -> (e4m3 codes uint8 [N][f8_stride(K)], fp32 scales [ceil(N / 128)][ceil(K / 128)]): one scale per
-    128 x 128 block, its largest magnitude / 448 (1 for a block of zeros). Bytes past K are zero."""
+    128 x 128 block, its largest magnitude / 448 (1 for a block of zeros). Bytes past K are zero. A code is the e4m3 value
+    nearest to w / scale; the kernels' quantiser multiplies by the scale's reciprocal, see `f8_codes`."""
     n, k = w.shape
     rows, cols = -(-n // F8_GROUP), -(-k // F8_GROUP)
     codes = np.zeros((n, f8_stride(k)), np.uint8)

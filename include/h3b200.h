@@ -292,8 +292,11 @@ H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages,
 /* ---- Block-scaled e4m3 linear layers -------------------------------------------------------------------------------
  * The second 8-bit number format beside int8: e4m3 codes with one fp32 scale per 128 channels of a row (activations)
  * or per 128 x 128 block (weights), without a rotation. No counterpart in the reference. For rows v[m][D]:
- *   s[g][m] = max(max_{k in group g} |v[m][k]| / 448, 2^-126), 1 where the group is all zero; code = e4m3(v / s),
- *   nearest, ties to even. G = ceil(D / 128) groups; a last group of D % 128 channels has a scale of its own.
+ *   s[g][m] = max(max_{k in group g} |v[m][k]| / 448, 2^-126), 1 where the group is all zero; code = e4m3(v * r) with
+ *   r = 1 / s, nearest, ties to even; s, r and v * r are each one fp32 rounding. That is the code nearest to v / s, but
+ *   where v / s lies within 2^-23 of itself of the middle between two codes it may be either of them (values of few bits
+ *   often do: one in 2000 of a bf16 row comes out otherwise than by a division). Weights prepared on the host (quant.py)
+ *   are divided by their scale. G = ceil(D / 128) groups; a last group of D % 128 channels has a scale of its own.
  * Codes are bytes [M][out_stride] (rows 16-byte aligned; bytes past D are not written), scales fp32
  * [G][sa_stride >= M]: a group's scales of all rows side by side. Any M, N, D, K >= 1. A NaN stays a NaN in its own
  * place; a group that holds an infinity reads back as NaN. Rows past M are neither read nor written.
@@ -301,7 +304,7 @@ H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages,
  *   h3b_rms_f8    h = x (+ y);  v = h / sqrt(mean(h^2) + eps) * w.   x [M][x_stride], w [D]; with y [M][y_stride] the sum h
  *                 is rounded to x's type, stored to res [M][res_stride] (x's type; res may be x) and then normed;
  *                 without y, res must be NULL. x, y, w of type bf16, f16 or f32 each. D <= 32768.
- *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D])
+ *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D]), to 115 * 2^-24 of itself at most
  *   h3b_gemm_f8   C[m][n] = c_dtype(sum_g sa[g][m] * sw[n / 128][g] * sum_{k in g} A[m][k] * W[n][k]  (+ bias[n]))
  *                 A codes [M][a_stride], W codes [N][w_stride] (K-contiguous, rows 16-byte aligned), sa as above,
  *                 sw fp32 [ceil(N / 128)][sw_stride >= G], bias fp32 [N] or NULL, C [M][c_stride] bf16, f16 or f32.
