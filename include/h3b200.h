@@ -304,7 +304,8 @@ H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages,
  *   h3b_rms_f8    h = x (+ y);  v = h / sqrt(mean(h^2) + eps) * w.   x [M][x_stride], w [D]; with y [M][y_stride] the sum h
  *                 is rounded to x's type, stored to res [M][res_stride] (x's type; res may be x) and then normed;
  *                 without y, res must be NULL. x, y, w of type bf16, f16 or f32 each. D <= 32768.
- *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D]), to 115 * 2^-24 of itself at most
+ *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D]); silu is off by 115 * 2^-24 of itself at most, and
+ *                 0 where e^-g passes the largest fp32 value (g < -88.7)
  *   h3b_gemm_f8   C[m][n] = c_dtype(sum_g sa[g][m] * sw[n / 128][g] * sum_{k in g} A[m][k] * W[n][k]  (+ bias[n]))
  *                 A codes [M][a_stride], W codes [N][w_stride] (K-contiguous, rows 16-byte aligned), sa as above,
  *                 sw fp32 [ceil(N / 128)][sw_stride >= G], bias fp32 [N] or NULL, C [M][c_stride] bf16, f16 or f32.
