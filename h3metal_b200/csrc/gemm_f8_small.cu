@@ -109,6 +109,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
     tmem_relinquish();
   }
   tc_fence_before_sync();
+  __syncwarp();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_holder;
@@ -236,6 +237,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
   // A][128]
   float *sums = reinterpret_cast<float *>(base_ptr);
   tc_fence_before_sync();
+  __syncwarp();  // warps 0 and 1 come from loops that lane 0 ran alone
   __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
@@ -245,7 +247,6 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
 #pragma unroll
     for (int j = 0; j < kRows; ++j) sums[(part * kRows + j) * kWRows + row] = acc[j];
   }
-  __syncwarp();
   cluster_sync_all();
   if (warp >= 2 && n < g.N && !*cta_abort) {
     // this CTA finishes the rows t = rank, rank + split, ..: its epilogue warps take them in turn
@@ -260,7 +261,6 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
       store_one(g, m0 + t, n, __fadd_rn(sum, bias));
     }
   }
-  __syncwarp();
   cluster_sync_all();  // nobody leaves while its sums are still being read
 }
 

@@ -149,15 +149,20 @@ __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.b
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ---- tensor memory ----------------------------------------------------------------------------------------------
-// Whole-warp calls. `cols` is a power of two in [32, 512]; the base address is written to shared memory.
+// Whole-warp calls. `cols` is a power of two in [32, 512]; the base address is written to shared memory. Instructions marked
+// .aligned need the warp's threads together, and a barrier only counts threads: behind a loop that one lane ran alone
+// nothing else brings them together again. So each of these calls starts with __syncwarp().
 __device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t cols) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(cols)
                : "memory");
 }
 __device__ __forceinline__ void tmem_relinquish() {
+  __syncwarp();
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before_sync() {
@@ -284,6 +289,7 @@ __device__ __forceinline__ uint32_t cluster_count_x() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // shared::cluster address of `local_addr` (a shared::cta address of this CTA) in CTA `rank` of the cluster
@@ -324,12 +330,15 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const CUtens
       : "memory");
 }
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t cols) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tmem_relinquish_pair() {
+  __syncwarp();
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
 // D[tmem of both CTAs] (+)= A * B^T with M = 256 spread over the pair; issued by ONE thread of the leader CTA.
