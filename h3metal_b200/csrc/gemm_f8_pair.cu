@@ -234,14 +234,14 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
 #pragma unroll
       for (int j = 0; j < kF8Cols / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
       // the next group's scales are fetched while this group's are waited for and used
-      float a_s = __ldg(g.sa + static_cast<size_t>(g_begin) * g.sa_stride + m_s);
-      float w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin);
+      float a_s = ld_f32(g.sa + static_cast<size_t>(g_begin) * g.sa_stride + m_s);
+      float w_s = ld_f32(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin);
 #pragma unroll 1
       for (int kb = 0; kb < groups; ++kb) {
         const float s = __fmul_rn(a_s, w_s);
         if (kb + 1 < groups) {
-          a_s = __ldg(g.sa + static_cast<size_t>(g_begin + kb + 1) * g.sa_stride + m_s);
-          w_s = __ldg(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin + kb + 1);
+          a_s = ld_f32(g.sa + static_cast<size_t>(g_begin + kb + 1) * g.sa_stride + m_s);
+          w_s = ld_f32(g.sw + static_cast<size_t>(n_s) * g.sw_stride + g_begin + kb + 1);
         }
         ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
         ok = __all_sync(0xFFFFFFFFu, ok);  // a warp gives up as a whole
@@ -295,7 +295,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
 #pragma unroll
       for (int j = 0; j < kF8Cols / 32; ++j) {
         const int n = n0 + j * 32 + lane;
-        bias[j] = g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
+        bias[j] = g.bias != nullptr && n < g.N ? ld_f32(g.bias + n) : 0.0f;
       }
       const int out_warp = SPLIT == 1 ? part * 4 + quarter : quarter;
       uint8_t *out_buf = base_ptr + P::kOutOff + out_warp * kF8OutWarp;

@@ -188,8 +188,8 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const bool have = g_begin + u < g_end;
-      a_s[u] = have ? __ldg(sa_p + static_cast<size_t>(g_begin + u) * g.sa_stride) : 0.0f;
-      w_s[u] = have ? __ldg(sw_p + g_begin + u) : 0.0f;
+      a_s[u] = have ? ld_f32(sa_p + static_cast<size_t>(g_begin + u) * g.sa_stride) : 0.0f;
+      w_s[u] = have ? ld_f32(sw_p + g_begin + u) : 0.0f;
     }
     RingPos pos, buf;
     bool ok = true;
@@ -201,8 +201,8 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
         float *slot = slots + (u & 1) * kRows;
         if (lane < kRows) slot[lane] = __fmul_rn(a_s[u], w_s[u]);
         if (kb + kAhead < g_end) {
-          a_s[u] = __ldg(sa_p + static_cast<size_t>(kb + kAhead) * g.sa_stride);
-          w_s[u] = __ldg(sw_p + kb + kAhead);
+          a_s[u] = ld_f32(sa_p + static_cast<size_t>(kb + kAhead) * g.sa_stride);
+          w_s[u] = ld_f32(sw_p + kb + kAhead);
         }
         __syncwarp();  // this slot is written, and every lane is done with the other one
         ok = mbar_wait(done_bar(pos.s), pos.ph, cta_abort, g.status, kStatusEpilogueTimeout);
@@ -231,7 +231,7 @@ gemm_f8_small_kernel(const __grid_constant__ GemmF8Launch g, const int stages, c
     }
   }
 
-  const float bias = warp >= 2 && g.bias != nullptr && n < g.N ? __ldg(g.bias + n) : 0.0f;
+  const float bias = warp >= 2 && g.bias != nullptr && n < g.N ? ld_f32(g.bias + n) : 0.0f;
   // Every copy has landed and every MMA has read it (the last group has been waited for by all epilogue warps before
   // any of them can pass the barrier below), so tensor memory can go and the ring holds the partial sums: [row of
   // A][128]

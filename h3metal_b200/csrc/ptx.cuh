@@ -103,6 +103,14 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // this kernel's CTAs free their resources. Both are no-ops for a kernel launched the ordinary way.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// What the kernel ahead may have written (activation scales, for one) is read by ordinary loads that stay behind
+// grid_dep_wait(): the read-only path (__ldg) is defined for memory that nobody writes while this kernel lives, and this kernel
+// may have been started before the one ahead had written it.
+__device__ __forceinline__ float ld_f32(const float *p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
 
 // ---- TMA ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_descriptor(const CUtensorMap *map) {

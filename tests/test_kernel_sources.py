@@ -46,3 +46,13 @@ def test_the_few_row_kernel_meets_its_barriers_with_whole_warps():
     text = source("gemm_f8_small.cu")
     for m in re.finditer(r"__syncthreads\(\);", text):
         assert text[:m.start()].rstrip().endswith("__syncwarp();")
+
+
+@pytest.mark.parametrize("name", ["gemm_f8_small.cu", "gemm_f8_pair.cu"])
+def test_scales_are_read_by_ordinary_loads(name):
+    """The product may start while the kernel that writes its activations' scales still runs: the read-only path is not defined
+    for such memory. ptx.cuh's ld_f32 is a volatile statement: it stays behind grid_dep_wait()."""
+    text = source(name)
+    assert "__ldg" not in text and "ld.global.nc" not in text and text.count("ld_f32(") >= 3
+    body = functions(source("ptx.cuh"))["ld_f32"]
+    assert "asm volatile" in body and "ld.global.f32" in body
