@@ -187,7 +187,7 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
         const uint64_t ad0 = umma_smem_desc(base, 1024, 2);
         const uint64_t bd0 = umma_smem_desc(base + kABytes, 1024, 2);
         RingPos pos, buf;
-        bool ok = true;
+        bool ok = true, issued = false;
         for (int tile = first_tile; ok && tile < num_tiles; tile += tile_step) {
           for (int kb = 0; kb < groups; ++kb) {
             const uint32_t s = pos.s;
@@ -205,7 +205,15 @@ gemm_f8_pair_kernel(const __grid_constant__ GemmF8Launch g) {
             umma_commit_pair(done_bar(s), static_cast<uint16_t>(3u << leader_cta));
             pos.advance(stages);
             buf.advance(2);
+            issued = true;
           }
+        }
+        if (*cta_abort && issued) {
+          // wind-down after a timeout: the last instructions issued must be done with both CTAs' shared and tensor memory
+          // before either gives them up
+          pos.retreat(stages);
+          int dummy_abort = 0;
+          mbar_wait(done_bar(pos.s), pos.ph, &dummy_abort, g.status, kStatusDrainTimeout, kDrainLimitCycles);
         }
       }
     }

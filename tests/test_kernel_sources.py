@@ -56,3 +56,13 @@ def test_scales_are_read_by_ordinary_loads(name):
     assert "__ldg" not in text and "ld.global.nc" not in text and text.count("ld_f32(") >= 3
     body = functions(source("ptx.cuh"))["ld_f32"]
     assert "asm volatile" in body and "ld.global.f32" in body
+
+
+@pytest.mark.parametrize("name", ["gemm_f8_small.cu", "gemm_f8_pair.cu"])
+def test_the_issuer_waits_for_its_instructions_when_a_wait_ran_out(name):
+    """Between the issuing loop and the end of the issuer's branch: a bounded wait on the stage that was committed last."""
+    text = source(name)
+    tail = text[text.index("umma_commit"):]
+    tail = tail[:tail.index("tmem_dealloc")]
+    assert re.search(r"if \(\*cta_abort && issued\) \{\s*pos\.retreat\(stages\);\s*int dummy_abort = 0;\s*"
+                     r"mbar_wait\(done_bar\(pos\.s\), pos\.ph, &dummy_abort", tail)
