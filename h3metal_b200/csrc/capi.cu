@@ -946,6 +946,17 @@ int h3b_gemm_f8(h3b_ctx *ctx, const h3b_gemm_f8_args *args) {
   return ctx->after_launch("gemm_f8 launch", h3b::launch_gemm_f8_small(g, ctx->prop.multiProcessorCount, ctx->stream));
 }
 
+int h3b_gemm_f8_kernel(h3b_ctx *ctx, int M, int N, int K) {
+  if (!ctx) return fail("null context");
+  if (M <= 0 || N <= 0 || K <= 0) return fail("gemm_f8: M, N and K must be positive");
+  if (ctx->f8_resident.pairs < 1) return fail("gemm_f8: the device holds no CTA pair of this kernel");
+  h3b::GemmF8Launch g;
+  memset(&g, 0, sizeof g);
+  g.M = M; g.N = N; g.K = K;
+  if (!h3b::gemm_f8_choose(g, ctx->prop.multiProcessorCount, ctx->f8_resident)) return g.nt;
+  return g.split == 1 ? 256 : 512;
+}
+
 int h3b_selftest_expire_wait(h3b_ctx *ctx) {
   if (!ctx) return fail("null context");
   cudaEvent_t ps = nullptr;

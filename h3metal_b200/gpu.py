@@ -89,6 +89,7 @@ def _signatures():
         "h3b_rms_f8": (i32, [vp, cp]),
         "h3b_quant_f8": (i32, [vp, cp]),
         "h3b_gemm_f8": (i32, [vp, cp]),
+        "h3b_gemm_f8_kernel": (i32, [vp, i32, i32, i32]),
         "h3b_gemm_tile_n": (i32, [vp, i32, i32]),
         "h3b_gemm_set_policy": (i32, [vp, i32, i32, i32]),
         "h3b_gemm_set_store_mode": (i32, [vp, i32]),
@@ -511,6 +512,14 @@ class Gpu:
                                                     c_stride, rows, N, row0, ctypes.c_void_p(rtype_ptr), gate.ptr, g_stride))
         if self._profile:
             self.names.append("reduce_dequant(epi1)")
+
+    def gemm_f8_kernel(self, M: int, N: int, K: int) -> int:
+        """The kernel gemm_f8 takes for these sizes: 16 / 32 / 64 / 128 few rows, that many to a tile; 256 CTA pairs; 512 two
+        pairs that share K."""
+        got = lib().h3b_gemm_f8_kernel(self.ctx, M, N, K)
+        if got < 0:
+            raise GpuError(_err())
+        return got
 
     def gemm_tile_n(self, N: int, lora: bool) -> int:
         return lib().h3b_gemm_tile_n(self.ctx, N, int(lora))

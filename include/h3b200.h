@@ -353,6 +353,9 @@ typedef struct {
 H3B_API int h3b_rms_f8(h3b_ctx *ctx, const h3b_rms_f8_args *args);
 H3B_API int h3b_quant_f8(h3b_ctx *ctx, const h3b_quant_f8_args *args);
 H3B_API int h3b_gemm_f8(h3b_ctx *ctx, const h3b_gemm_f8_args *args);
+/* Which kernel a product of these sizes takes: 16, 32, 64 or 128 (the few-row kernel and its rows of A per tile), 256 (CTA
+ * pairs) or 512 (two pairs share K). Negative on error. Launches nothing. */
+H3B_API int h3b_gemm_f8_kernel(h3b_ctx *ctx, int M, int N, int K);
 
 /* Self-test of the error path the kernels share. Every device-side wait in this library is bounded: when one runs
  * out the kernel records a code in the context's status word, winds down and returns, and the next h3b_wait reports
