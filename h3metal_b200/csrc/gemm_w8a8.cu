@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(64 + 32 * EPI_WARPS, 1) gemm_w8a8_kernel(const
       float *sw_s = col_stage + (warp - 2) * 2 * BN, *bias_s = sw_s + BN;
       stage_columns(g, n0, BN, lane, sw_s, bias_s);
       const int m = m0 + row;
-      const float sa_m = (!raw && m < g.M) ? __ldg(g.sa + m) : 0.0f;
+      const float sa_m = (!raw && m < g.M) ? ld_f32(g.sa + m) : 0.0f;
       bool has_low = false;
       if (LORA) {
         int k0 = 0, k1 = g.R;

@@ -264,7 +264,7 @@ gemm_w8a8_pair_kernel(const __grid_constant__ GemmLaunch g, const int stages) {
       float *sw_s = col_stage + (warp - 2) * 2 * kWarpCols, *bias_s = sw_s + kWarpCols;  // this warp's columns only
       stage_columns(g, n0 + part * kWarpCols, kWarpCols, lane, sw_s, bias_s);
       const int m = m0 + row;
-      const float sa_m = (!raw && m < g.M) ? __ldg(g.sa + m) : 0.0f;
+      const float sa_m = (!raw && m < g.M) ? ld_f32(g.sa + m) : 0.0f;
       bool has_low = false;
       if (LORA) {
         int k0 = 0, k1 = g.R;

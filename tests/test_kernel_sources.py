@@ -66,3 +66,9 @@ def test_the_issuer_waits_for_its_instructions_when_a_wait_ran_out(name):
     tail = tail[:tail.index("tmem_dealloc")]
     assert re.search(r"if \(\*cta_abort && issued\) \{\s*pos\.retreat\(stages\);\s*int dummy_abort = 0;\s*"
                      r"mbar_wait\(done_bar\(pos\.s\), pos\.ph, &dummy_abort", tail)
+
+
+@pytest.mark.parametrize("name", ["gemm_w8a8.cu", "gemm_w8a8_pair.cu"])
+def test_the_int8_product_reads_its_activations_scales_the_same_way(name):
+    text = source(name)
+    assert "ld_f32(g.sa" in text and not re.search(r"__ldg\(g\.sa\b", text)
