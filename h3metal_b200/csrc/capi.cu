@@ -849,6 +849,7 @@ int h3b_quant_f8(h3b_ctx *ctx, const h3b_quant_f8_args *args) {
   if (sa_stride < M) return fail("quant_f8: sa_stride smaller than M");
   if (!rows_aligned(x, x_stride, size) || !rows_aligned(out, out_stride, 1))
     return fail("quant_f8: rows must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(sa) % 4) return fail("quant_f8: sa is not aligned to its elements");
   if (D > (1 << 28)) return fail("quant_f8: D exceeds 2^28 channels");
   h3b::QuantF8Launch q;
   q.x = x; q.out = out; q.sa = sa; q.x_stride = x_stride; q.out_stride = out_stride; q.sa_stride = sa_stride;
@@ -875,6 +876,7 @@ int h3b_rms_f8(h3b_ctx *ctx, const h3b_rms_f8_args *args) {
   if (!rows_aligned(x, x_stride, sx) || !rows_aligned(out, out_stride, 1) || !rows_aligned(w, 0, 1) ||
       (y && (!rows_aligned(y, y_stride, sy) || !rows_aligned(res, res_stride, sx))))
     return fail("rms_f8: rows must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(sa) % 4) return fail("rms_f8: sa is not aligned to its elements");
   if (!(eps >= 0.0f)) return fail("rms_f8: eps must not be negative");
   h3b::RmsF8Launch r;
   r.x = x; r.y = y; r.w = w; r.res = res; r.out = out; r.sa = sa;
