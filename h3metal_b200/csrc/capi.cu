@@ -850,7 +850,7 @@ int h3b_quant_f8(h3b_ctx *ctx, const h3b_quant_f8_args *args) {
   if (!rows_aligned(x, x_stride, size) || !rows_aligned(out, out_stride, 1))
     return fail("quant_f8: rows must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(sa) % 4) return fail("quant_f8: sa is not aligned to its elements");
-  if (D > (1 << 28)) return fail("quant_f8: D exceeds 2^28 channels");
+  if (D > h3b::kQuantF8MaxD) return fail("quant_f8: D exceeds the 2^28 - 4096 channels one launch covers");
   h3b::QuantF8Launch q;
   q.x = x; q.out = out; q.sa = sa; q.x_stride = x_stride; q.out_stride = out_stride; q.sa_stride = sa_stride;
   q.x_dtype = x_dtype; q.M = M; q.D = D; q.gated = mode;

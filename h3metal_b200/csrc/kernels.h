@@ -172,6 +172,7 @@ struct QuantF8Launch {
   long long x_stride, out_stride, sa_stride;
   int x_dtype, M, D, gated;
 };
+constexpr int kQuantF8MaxD = 65535 * 256 * 16;  // grid.y parts of 256 threads of 16 channels
 cudaError_t launch_quant_f8(const QuantF8Launch &q, bool overlap, cudaStream_t stream);
 
 struct RmsF8Launch {

@@ -395,7 +395,6 @@ cudaError_t launch_quant(const QuantF8Launch &q, bool overlap, cudaStream_t stre
     ty = 256 / tx;
   }
   const dim3 grid((q.M - 1) / ty + 1, (pieces + tx - 1) / tx), threads(tx, ty);
-  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
   if (q.gated) return launch(quant_f8_kernel<T, true>, grid, threads, overlap, stream, a);
   return launch(quant_f8_kernel<T, false>, grid, threads, overlap, stream, a);
 }

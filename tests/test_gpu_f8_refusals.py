@@ -26,3 +26,11 @@ def test_scales_off_their_alignment(gpu, rows, offset):
     sa = rows["sa"].view((12 * M,), "u8", offset).view((2, M), "f32")
     refused(gpu, lambda: gpu.quant_f8_native(x, D, out, D, sa, M, M, D, 0))
     refused(gpu, lambda: gpu.rms_f8_native(x, D, None, 0, None, 0, w, out, D, sa, M, M, D, 1e-6))
+
+
+def test_more_channels_than_a_launch_covers(gpu, rows):
+    """Turned down by its size alone: the buffers behind the pointers are never touched."""
+    x, out, sa = rows["x"], rows["out"], rows["sa"]
+    with pytest.raises(GpuError, match="channels one launch covers"):
+        gpu.quant_f8_native(x, 2 ** 28, out, 2 ** 28, sa, 1, 1, 2 ** 28 - 4095, 0)
+    refused(gpu, lambda: gpu.quant_f8_native(x, 2 ** 28, out, 2 ** 28, sa, 1, 1, 2 ** 28, 0))
