@@ -878,6 +878,9 @@ int h3b_rms_f8(h3b_ctx *ctx, const h3b_rms_f8_args *args) {
     return fail("rms_f8: rows must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(sa) % 4) return fail("rms_f8: sa is not aligned to its elements");
   if (!(eps >= 0.0f)) return fail("rms_f8: eps must not be negative");
+  // the sum may go where an addend was, value by value; laid out otherwise it would run over rows that are still to be read
+  if (y && ((res == x && M > 1 && res_stride != x_stride) || (res == y && (sx != sy || (M > 1 && res_stride != y_stride)))))
+    return fail("rms_f8: res may be x or y only in the same place: the same row stride and element size");
   h3b::RmsF8Launch r;
   r.x = x; r.y = y; r.w = w; r.res = res; r.out = out; r.sa = sa;
   r.x_stride = x_stride; r.y_stride = y_stride; r.res_stride = res_stride; r.out_stride = out_stride; r.sa_stride = sa_stride;

@@ -18,7 +18,7 @@ from dataclasses import dataclass, field, replace
 
 import numpy as np
 
-from .gpu import Gpu, Tensor, pack  # noqa: F401  (pack is re-exported like in the reference)
+from .gpu import _SIZE, Gpu, Tensor, pack  # noqa: F401  (pack is re-exported like in the reference)
 from .quant import F8_GROUP, RB, f8_stride
 
 FMT_ID = {"q8": 1, "q4": 2, "q4g": 3, "f16": 4, "bf16": 5, "h8": 6, "h4": 7, "h4g": 8}
@@ -295,7 +295,7 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
            res: Tensor | None = None, x_stride: int | None = None, y_stride: int | None = None, res_stride: int | None = None,
            out_stride: int | None = None, sa_stride: int | None = None):
     """out, sa = e4m3 codes and scales of rmsnorm(x) * w (w [D], no offset). With y, first x + y, rounded to x's type and
-    kept in res (x itself by default), is what is normed. x, y and w are bf16, f16 or f32, each its own. out: "f8" rows of
+    kept in res (x itself by default; x or y in their own place or memory apart from both), is what is normed. x, y and w are bf16, f16 or f32, each its own. out: "f8" rows of
     quant.f8_stride(D) bytes; sa: fp32 [ceil(D / 128)][M], a group's scales of all rows side by side. A code is
     e4m3(v * (1 / scale)) in fp32 steps (quant.f8_codes)."""
     if M <= 0 or D <= 0:
@@ -317,6 +317,9 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
         if res is None:
             res, res_stride = x, res_stride or x_stride
         y_stride, res_stride = y_stride or D, res_stride or D
+        for t, stride in ((x, x_stride), (y, y_stride)):
+            if res.ptr == t.ptr and (_SIZE[res.dtype] != _SIZE[t.dtype] or M > 1 and res_stride != stride):
+                raise ValueError("rms_f8: res may be x or y only in the same place: the same row stride and element size")
         if not _holds(y, _FLOATS, M, D, y_stride):
             _refuse("rms_f8 y", y, _FLOATS, M, D, y_stride)
         if not _holds(res, (x.dtype,), M, D, res_stride):

@@ -299,12 +299,11 @@ H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages,
  *   are divided by their scale. G = ceil(D / 128) groups; a last group of D % 128 channels has a scale of its own.
  * Codes are bytes [M][out_stride] (rows 16-byte aligned; bytes past D are not written), scales fp32
  * [G][sa_stride >= M]: a group's scales of all rows side by side. Any M, N, D, K >= 1 (rms_f8: D <= 32768; quant_f8:
- * D <= 2^28 - 4096). A NaN stays a NaN in its own
- * place; a group that holds an infinity reads back as NaN. Rows past M are neither read nor written.
+ * D <= 2^28 - 4096). A NaN stays a NaN in its own place; a group that holds an infinity reads back as NaN. Rows past M are neither read nor written.
  *
  *   h3b_rms_f8    h = x (+ y);  v = h / sqrt(mean(h^2) + eps) * w.   x [M][x_stride], w [D]; with y [M][y_stride] the sum h
- *                 is rounded to x's type, stored to res [M][res_stride] (x's type; res may be x) and then normed;
- *                 without y, res must be NULL. x, y, w of type bf16, f16 or f32 each.
+ *                 is rounded to x's type, stored to res [M][res_stride] (x's type) and then normed; res may be x or y themselves
+ *                 (same row stride and element size), else it overlaps neither. Without y, res must be NULL. x, y, w of type bf16, f16 or f32 each.
  *   h3b_quant_f8  mode 0: v = x;  mode 1: v = x[:, :D] * silu(x[:, D:2D]); silu is off by 115 * 2^-24 of itself at most, and
  *                 0 where e^-g passes the largest fp32 value (g < -88.7)
  *   h3b_gemm_f8   C[m][n] = c_dtype(sum_g sa[g][m] * sw[n / 128][g] * sum_{k in g} A[m][k] * W[n][k]  (+ bias[n]))
