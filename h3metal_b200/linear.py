@@ -56,16 +56,21 @@ def upload_weight_f8(gpu: Gpu, w: np.ndarray, bias=None) -> ops.QWeight:
 class BlockScaledLinear:
     """y = x W^T (+ bias) with e4m3 codes and block scales on both sides, for up to M rows: the quantiser (plain rows, or
     value | gate with swiglu_in) or, through normed(), the residual addition and RMSNorm in front of it, then the
-    product. Owns its buffers; a call may use fewer rows than M."""
+    product. Owns its buffers; a call may use fewer rows than M. Input rows start on 16-byte boundaries: where a width is
+    no multiple of that, rows lie apart (x_stride, and out_stride of the layer whose output they are)."""
 
-    def __init__(self, gpu: Gpu, wt: ops.QWeight, M: int, *, swiglu_in: bool = False, out_dtype: str = "bf16"):
+    def __init__(self, gpu: Gpu, wt: ops.QWeight, M: int, *, swiglu_in: bool = False, out_dtype: str = "bf16",
+                 out_stride: int | None = None):
         self.gpu, self.wt, self.M, self.swiglu_in = gpu, wt, M, swiglu_in
+        self.out_stride = wt.N if out_stride is None else out_stride
+        if self.out_stride < wt.N:
+            raise ValueError(f"out_stride {out_stride} is smaller than the {wt.N} columns of the output")
         self.codes = gpu.empty((M, quant.f8_stride(wt.K)), "f8")
         self.sa = gpu.empty((-(-wt.K // quant.F8_GROUP), M), "f32")
-        self.out = gpu.empty((M, wt.N), out_dtype)
+        self.out = gpu.empty((M, self.out_stride), out_dtype)
 
     def _product(self, M: int) -> Tensor:
-        ops.gemm_f8(self.gpu, self.codes, self.wt, self.out, M, sa=self.sa, sa_stride=self.M)
+        ops.gemm_f8(self.gpu, self.codes, self.wt, self.out, M, sa=self.sa, sa_stride=self.M, c_stride=self.out_stride)
         return self.out
 
     def _rows(self, M: int | None) -> int:
@@ -81,12 +86,14 @@ class BlockScaledLinear:
         return self._product(M)
 
     def normed(self, x: Tensor, gain: Tensor, M: int | None = None, *, eps: float, y: Tensor | None = None,
-               res: Tensor | None = None) -> Tensor:
+               res: Tensor | None = None, x_stride: int | None = None, y_stride: int | None = None,
+               res_stride: int | None = None) -> Tensor:
         """The layer behind an RMSNorm: x (+ y, the sum kept in res or in x itself) is normed, coded and multiplied."""
         if self.swiglu_in:
             raise ValueError("normed: a layer behind a gated activation has no norm in front of it")
         M = self._rows(M)
-        ops.rms_f8(self.gpu, x, gain, self.codes, self.sa, M, self.wt.K, eps=eps, y=y, res=res, sa_stride=self.M)
+        ops.rms_f8(self.gpu, x, gain, self.codes, self.sa, M, self.wt.K, eps=eps, y=y, res=res, x_stride=x_stride,
+                   y_stride=y_stride, res_stride=res_stride, sa_stride=self.M)
         return self._product(M)
 
     @property

@@ -297,7 +297,8 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
     """out, sa = e4m3 codes and scales of rmsnorm(x) * w (w [D], no offset). With y, first x + y, rounded to x's type and
     kept in res (x itself by default; x or y in their own place or memory apart from both), is what is normed. x, y and w are bf16, f16 or f32, each its own. out: "f8" rows of
     quant.f8_stride(D) bytes; sa: fp32 [ceil(D / 128)][M], a group's scales of all rows side by side. A code is
-    e4m3(v * (1 / scale)) in fp32 steps (quant.f8_codes)."""
+    e4m3(v * (1 / scale)) in fp32 steps (quant.f8_codes). Rows of x, y, res and out and w itself start on 16-byte boundaries:
+    a width of another multiple needs a stride of its own."""
     if M <= 0 or D <= 0:
         raise ValueError("rms_f8: M and D must be positive")
     x_stride, out_stride, sa_stride = x_stride or D, out_stride or f8_stride(D), sa_stride or M
@@ -330,8 +331,8 @@ def rms_f8(gpu: Gpu, x: Tensor, w: Tensor, out: Tensor, sa: Tensor, M: int, D: i
 
 def quant_f8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor, M: int, D: int, *, swiglu: bool = False,
              x_stride: int | None = None, out_stride: int | None = None, sa_stride: int | None = None):
-    """out, sa = e4m3 codes and scales of x (or of value * silu(gate) with the gates in columns D..2D-1); layouts as in
-    rms_f8."""
+    """out, sa = e4m3 codes and scales of x (or of value * silu(gate) with the gates in columns D..2D-1); layouts and
+    boundaries as in rms_f8 (the gates may start anywhere)."""
     if M <= 0 or D <= 0:
         raise ValueError("quant_f8: M and D must be positive")
     wide = 2 * D if swiglu else D

@@ -297,7 +297,8 @@ H3B_API int h3b_rot_set_policy(h3b_ctx *ctx, int threads_target, int tma_stages,
  *   where v / s lies within 2^-23 of itself of the middle between two codes it may be either of them (values of few bits
  *   often do: one in 2000 of a bf16 row comes out otherwise than by a division). Weights prepared on the host (quant.py)
  *   are divided by their scale. G = ceil(D / 128) groups; a last group of D % 128 channels has a scale of its own.
- * Codes are bytes [M][out_stride] (rows 16-byte aligned; bytes past D are not written), scales fp32
+ * Rows of x, y, res and of codes start on 16-byte boundaries (base and row stride), and so does w; the gates, C, bias and
+ * scales on those of their elements. Codes are bytes [M][out_stride] (bytes past D are not written), scales fp32
  * [G][sa_stride >= M]: a group's scales of all rows side by side. Any M, N, D, K >= 1 (rms_f8: D <= 32768; quant_f8:
  * D <= 2^28 - 4096). A NaN stays a NaN in its own place; a group that holds an infinity reads back as NaN. Rows past M are neither read nor written.
  *
