@@ -1,4 +1,4 @@
-"""The .h3m weight container, reading and writing, for the int8 linear path.
+"""The .h3m weight container, reading and writing, for the 8-bit linear paths.
 
 Same file format as the reference's h3metal/weights.py (layout :1-18, Writer :51-128, read_header :131-138,
 WeightFile :141-202), so files produced by the reference's converters can be read here and vice versa:
@@ -8,7 +8,8 @@ WeightFile :141-202), so files produced by the reference's converters can be rea
 Every tensor starts on a 256-byte boundary and does not cross a multiple of the chunk size (1 GiB) unless it is
 marked host-only. The JSON header maps names to entries: a plain tensor is {"offset", "nbytes", "shape", "dtype"};
 a linear layer is {"kind": "linear", "fmt", "N", "K", "G", "w": {...}, "sw": {...}, "bias": {...}}; "meta" carries
-the model configuration and "chunk" the chunk size.
+the model configuration and "chunk" the chunk size. Layers of fmt "f8" (e4m3 codes [N][f8_stride(K)] with one scale per
+128 x 128 block) are this library's own: the reference's reader does not know them.
 
 What differs from the reference is where the bytes go: the reference maps the file and hands the mapping to the GPU
 without copying (Apple's unified memory); a B200 has its own memory, so `WeightFile` maps the file on the host and
@@ -25,6 +26,7 @@ import struct
 
 import numpy as np
 
+from . import quant
 from .gpu import Gpu, Tensor
 from .ops import QWeight
 
@@ -35,12 +37,17 @@ CHUNK = 1 << 30
 ALIGN = 256
 
 _NP = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "i8": np.int8, "u8": np.uint8, "i32": np.int32,
-       "u16": np.uint16}
-_CODE_DTYPE = {"q8": "i8", "h8": "i8", "f16": "f16", "bf16": "bf16"}
+       "u16": np.uint16, "f8": np.uint8}
+_CODE_DTYPE = {"q8": "i8", "h8": "i8", "f16": "f16", "bf16": "bf16", "f8": "f8"}
 
 
 def _align(x: int) -> int:
     return -(-x // ALIGN) * ALIGN
+
+
+def _f8_shapes(N: int, K: int):
+    """Shapes of the codes and scales of an "f8" layer."""
+    return (N, quant.f8_stride(K)), (-(-N // quant.F8_GROUP), -(-K // quant.F8_GROUP))
 
 
 class Writer:
@@ -90,6 +97,10 @@ class Writer:
 
     def linear(self, name: str, fmt: str, N: int, K: int, w: np.ndarray, sw: np.ndarray | None,
                bias: np.ndarray | None = None, G: int = 128, extra: dict | None = None):
+        if fmt == "f8":  # rows of f8_stride(K) bytes and a scale per block: what linear() will look for
+            codes, scales = _f8_shapes(N, K)
+            if w.shape != codes or w.dtype.itemsize != 1 or sw is None or np.shape(sw) != scales or G != quant.F8_GROUP:
+                raise ValueError(f"{name}: e4m3 codes {codes} of bytes and scales {scales} are wanted for {N} x {K}")
         entry = {"kind": "linear", "fmt": fmt, "N": N, "K": K, "G": G, "w": self._put(w)}
         if sw is not None:
             entry["sw"] = self._put(np.asarray(sw, dtype=np.float32))
@@ -159,9 +170,10 @@ class WeightFile:
         e = self.entries[name]
         fmt, N, K = e["fmt"], e["N"], e["K"]
         if fmt not in _CODE_DTYPE:
-            raise NotImplementedError(f"{name}: weight format {fmt!r} is outside the int8 linear path")
-        w = self._device(e["w"], (N, K), _CODE_DTYPE[fmt])
-        sw = self._device(e["sw"], (e["sw"]["nbytes"] // 4,), "f32") if "sw" in e else None
+            raise NotImplementedError(f"{name}: weight format {fmt!r} is outside the 8-bit linear path")
+        codes, scales = _f8_shapes(N, K) if fmt == "f8" else ((N, K), (e["sw"]["nbytes"] // 4,) if "sw" in e else None)
+        w = self._device(e["w"], codes, _CODE_DTYPE[fmt])
+        sw = self._device(e["sw"], scales, "f32") if "sw" in e else None
         bias = self._device(e["bias"], (N,), "f32") if "bias" in e else None
         return QWeight(fmt, w, sw, N, K, e.get("G", 128), bias)
 
