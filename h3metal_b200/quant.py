@@ -138,7 +138,8 @@ def f8_codes(v: np.ndarray, s: np.ndarray) -> np.ndarray:
 
 def quant_f8(w: np.ndarray):
     """Weight [N][K] -> (e4m3 codes uint8 [N][f8_stride(K)], fp32 scales [ceil(N / 128)][ceil(K / 128)]): one scale per
-    128 x 128 block, its largest magnitude / 448 (1 for a block of zeros). Bytes past K are zero. A code is the e4m3 value
+    128 x 128 block, its largest magnitude / 448 (1 for a block of zeros). A NaN keeps its own place, and its block's scale comes
+    from the other values; a block that holds an infinity reads back as NaN. Bytes past K are zero. A code is the e4m3 value
     nearest to w / scale; the kernels' quantiser multiplies by the scale's reciprocal, see `f8_codes`."""
     n, k = w.shape
     rows, cols = -(-n // F8_GROUP), -(-k // F8_GROUP)
@@ -149,9 +150,10 @@ def quant_f8(w: np.ndarray):
         full = np.zeros((len(band), cols * F8_GROUP), np.float32)
         full[:, :k] = band
         blocks = full.reshape(len(band), cols, F8_GROUP)
-        top = np.abs(blocks).max(axis=(0, 2))
+        top = np.fmax.reduce(np.abs(blocks), axis=(0, 2), initial=np.float32(0))  # a NaN is left out, as in the kernels
         scales[i] = np.where(top > 0, np.maximum(top / np.float32(F8_TOP), np.float32(_F8_TINY)), np.float32(1.0))
-        codes[i * F8_GROUP:(i + 1) * F8_GROUP, :k] = e4m3_bits(blocks / scales[i][None, :, None]).reshape(len(band), -1)[:, :k]
+        with np.errstate(invalid="ignore"):  # a block that holds an infinity reads back as NaN
+            codes[i * F8_GROUP:(i + 1) * F8_GROUP, :k] = e4m3_bits(blocks / scales[i][None, :, None]).reshape(len(band), -1)[:, :k]
     return codes, scales
 
 
