@@ -23,7 +23,8 @@ def refused(gpu, call):
 @pytest.mark.parametrize("offset", [1, 2, 3])
 def test_scales_off_their_alignment(gpu, rows, offset):
     M, D, x, w, out = (rows[k] for k in ("M", "D", "x", "w", "out"))
-    sa = rows["sa"].view((12 * M,), "u8", offset).view((2, M), "f32")
+    sa = rows["sa"].view((12 * M,), "u8").view((8 * M,), "u8", offset).view((2, M), "f32")
+    assert sa.ptr % 4 == offset
     refused(gpu, lambda: gpu.quant_f8_native(x, D, out, D, sa, M, M, D, 0))
     refused(gpu, lambda: gpu.rms_f8_native(x, D, None, 0, None, 0, w, out, D, sa, M, M, D, 1e-6))
 
