@@ -8,10 +8,11 @@
 //
 // What bounds it: a group's MMAs take 512 cycles; reading it out of tensor memory, 128 x 256 values per SM, and the
 // multiply-adds (two columns per packed instruction) take about 250 each, beside the MMAs of the next group, for
-// which there is a second accumulator of 256 columns. An accumulator goes round through the pair (MMAs done -> both
-// epilogues -> leader), and two messages between SMs cost 0.6 us, so a group takes 860 cycles. Measured, back to back
-// for a second under the board's power cap: 17408 x 18432 x 6144 in 1.87 ms = 2.10 PFLOP/s at 1.46 GHz, 9.7 of 16.4
-// kflop per clock and SM (60 %); three launches from idle 2.39 PFLOP/s. With an epilogue that only hands accumulators
+// which there is a second accumulator of 256 columns. An accumulator goes round (MMAs done -> both epilogues -> leader), and
+// a group takes 860 to 900 cycles, with no pipe near its limit: latency somewhere in that round, where is not
+// measured. Messages between the two SMs are not all of it, since single CTAs, which send none, are no faster. Measured, back
+// to back under the board's power cap: 17408 x 18432 x 6144 in 1.87 to 1.91 ms = 2.06 to 2.10 PFLOP/s at 1.46 GHz, 9.7 of
+// 16.4 kflop per clock and SM (60 %); three launches from idle 2.39 PFLOP/s. With an epilogue that only hands accumulators
 // back: 2.24; without its multiply-adds: 2.27. Not taken: three accumulators of 160 columns (2.48 against 1.96 ms:
 // more bytes per multiply, and the issuing thread's four instructions and commit per group no longer hide), MMAs of
 // 128 columns into four accumulators (+17 %: A is read twice from shared memory), single CTAs on 128 x 256 tiles (+10

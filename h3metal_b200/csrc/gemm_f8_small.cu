@@ -15,9 +15,10 @@
 // four lane quarters x parts of up to 32 rows of A. Out-of-range rows and channels are zero-filled by TMA. All waits
 // are bounded. No load uses multicast.
 //
-// What bounds it: HBM for few rows. 1 x 11520 x 3840, one of a chain of launches: 9.8 us = 4.5 TB/s; the weights
-// themselves stream at 6.2 TB/s for 7.1 us of them, the rest is the first tile's latency (1.3 us), the two cluster
-// barriers and the exit. For 64 and more rows the one issuing thread: two barrier polls, four instructions and a
+// What bounds it: HBM for few rows. In a chain of launches whose weights rotate through 354 MB, so that each comes from HBM
+// (44.3 MB of DRAM reads per launch counted): 1 x 11520 x 3840 10.2 us = 4.3 TB/s, 16 x 3840 x 10240 10.3 us; with the
+// weights of the launch before in L2 8.9 and 8.6 us. What is not the weights' way is the first tile's latency (1.3 us), the two
+// cluster barriers and the exit. For 64 and more rows the one issuing thread: two barrier polls, four instructions and a
 // commit take 600 to 850 cycles per group.
 #include <cuda.h>
 
@@ -311,7 +312,7 @@ cudaError_t launch_nt(const GemmF8Launch &g, int sms, cudaStream_t stream) {
 // that share K pay 1.5 us to meet, and take one tile per cluster. M x N x K: here / a pair / two pairs, us: 256 x 3840
 // x 3840: 15.2 / 17.4 / 13.8; 512 x 3840 x 10240: 42.4 / 37.8 / 26.8; 128 x 3840 x 3840: 10.4 / 17 / 13.6; 128 x 20480
 // x 3840: 44.6 / 33.2; 512 x 20480 x 3840: 97 / 47. Over nine M of 1 to 640 and seven N x K the choice is within 2 % of
-// the best.
+// the best; larger products were not swept.
 bool gemm_f8_choose(GemmF8Launch &g, int sms, const F8Clusters &resident) {
   const long long groups = (g.K + kBKBytes - 1) / kBKBytes;
   const long long n_tiles = (static_cast<long long>(g.N) + kWRows - 1) / kWRows;

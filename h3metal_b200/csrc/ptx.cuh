@@ -142,8 +142,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const CUtensorMap
 }
 
 // 2-D tile store shared -> global (this GPU's memory), tracked by the thread's bulk groups. x is the innermost
-// coordinate in elements and must keep the destination 16-byte aligned; rows or columns beyond the tensor's
-// extents are not written. The shared-memory source must have been made visible to the asynchronous proxy
+// coordinate in elements and must keep the destination 16-byte aligned; rows beyond the tensor's extents are
+// not written, and columns beyond them in whole 16-byte pieces only (a row must end on such a boundary). The shared-memory source must have been made visible to the asynchronous proxy
 // (fence_proxy_async_smem) by the threads that wrote it.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src_smem, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"

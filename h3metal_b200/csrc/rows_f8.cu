@@ -14,10 +14,14 @@
 //
 // A thread owns a piece of 16 channels (one 16-byte store of codes), eight neighbouring lanes a group of 128: the
 // group's largest magnitude is three shuffles. Both kernels are bound by memory: 1 byte written per channel beside
-// the 2 to 10 read and kept. Measured: quant_f8 17408 x 16384 gated, 1.43 GB in 208 us = 6.9 TB/s (the measured copy
-// rate is 6.55), 17408 x 6144 plain 52 us = 6.2 TB/s; rms_f8 17408 x 6144 with a bf16 stream and addend 119 us = 6.3
-// TB/s, with an fp32 stream 205 us = 5.8, 4608 x 3840 24 us = 5.1 (a tenth of it launch and first rows), without an
-// addend 69 us = 4.7 (the chain of a row's sum, not memory).
+// the 2 to 10 read and kept. Measured as a chain of launches over more than L2 holds (the measured copy rate is 6.55 TB/s):
+// quant_f8 17408 x 16384 gated, 1.43 GB in 208 us = 6.9 TB/s (222 us called one by one from Python), 17408 x 6144 plain
+// 52 us = 6.2 TB/s; rms_f8 17408 x 6144 with a bf16 stream and addend 118 us = 6.4 TB/s, with an fp32 stream 209 us = 5.6,
+// 4608 x 3840 24 us = 5.2 (a tenth of it launch and first rows), bf16 without an addend 69 us = 4.7 and fp32 83 us = 6.5
+// (the chain of a row's sum shows where there are few bytes). Where registers do not reach the row loop spills: two fp32
+// inputs (172 bytes of spill stores; 17408 x 6144 258 us = 5.4 TB/s), and D of 8193 to 16384 with an addend, where 1024
+// threads leave 64 each (192 to 356 bytes; 4096 x 16384: bf16 88 us = 5.4, fp32 stream 126 us = 5.9, both fp32 204 us = 4.3);
+// beyond, rows of four pieces per thread without the next row on its way (4096 x 32768 bf16 228 us = 4.1).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
